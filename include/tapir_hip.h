@@ -394,6 +394,75 @@ int tapir_xconv(tapir_ctx* ctx, const void* x, const void* wstream, const float*
 int tapir_xconv_nt(tapir_ctx* ctx, const void* x, const void* wstream, const float* bias, const void* skip,
                    void* y, int N, int H, int W, int cin, int cout, int gelu, int form, void* stream);
 
+/* Layer normalisation, rotary positions and cross attention: what a learned readout of the feature grids consists of
+ * (points attend to a clip's cells).  No counterpart in tapnet's TAPIR; the Python forms are in tapnet_amd/attention.py.
+ * Tensors are in the context's element type, everything else is f32 unless stated.  No weights are needed
+ * (tapir_finalize_weights may be left out), nothing is kept between calls, and the context's own workspaces are not
+ * used: scratch memory is the caller's (`workspace`, 16-byte aligned, as many bytes as the ..._workspace call says, free
+ * again when the work on `stream` is done), so that calls on different streams and captured graphs share nothing.
+ * Results do not depend on the run: there are no atomics. */
+
+/* y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis.  x [rows, channels] with `x_stride` elements from
+ * row to row, y dense; gamma / beta [channels] or NULL (ones / zeros); mean, rstd [rows] are written where both are
+ * given (the backward pass needs them).  Any channel count; rows of whole 16-byte multiples that start at such
+ * addresses are read and written 16 bytes at a time. */
+int tapir_layer_norm(tapir_ctx* ctx, const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y,
+                     float* mean, float* rstd, int64_t rows, int channels, float eps, void* stream);
+/* dx (dense), dgamma, dbeta [channels] (either may be NULL; they are overwritten, not added to). */
+int tapir_layer_norm_workspace(tapir_ctx* ctx, int64_t rows, int channels, uint64_t* bytes);
+int tapir_layer_norm_backward(tapir_ctx* ctx, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,
+                              const float* gamma, const float* mean, const float* rstd, void* dx, float* dgamma,
+                              float* dbeta, int64_t rows, int channels, void* workspace, uint64_t workspace_bytes,
+                              void* stream);
+
+/* Rotary positions of up to 4 axes.  The first section[0] channels of a head belong to axis 0, the next section[1] to
+ * axis 1 ..., channels behind the last section are copied.  Pair i of a section of width w turns by
+ * position * base^(-2 i / w); its channels are 2 i, 2 i + 1 of the section (interleaved) or i, i + w / 2.  `inverse`
+ * turns back (the gradient).  x [batch, tokens, heads, dim] with strides (clip, token, head) in elements and dense
+ * channels, positions [batch or 1, tokens, axes] dense with positions_stride elements from clip to clip (0: the same for
+ * all), y dense.  dim <= 256.  Angles are formed in 64 bits. */
+typedef struct tapir_rotary_args {
+  int64_t batch, tokens;
+  int heads, dim, axes, interleaved, inverse;
+  int section[4];
+  double base[4];
+  const void* x;
+  int64_t x_stride[3];
+  const float* positions;
+  int64_t positions_stride;
+  void* y;
+} tapir_rotary_args;
+int tapir_rotary_positions(tapir_ctx* ctx, const tapir_rotary_args* args, void* stream);
+
+/* softmax(scale q k^T) v of query rows over an encoder's tokens.  q [batch, queries, heads, dim], k and v [batch, keys,
+ * kv_heads, dim], heads a multiple of kv_heads (query head j reads key head j / (heads / kv_heads)); strides (clip,
+ * token, head) in elements, channels dense, every row at a multiple of 16 bytes; dim a multiple of 8, at most 128;
+ * scale > 0.  key_lengths [batch] int32 (device; clamped to 0 .. keys) and key_mask [batch, keys] bytes (nonzero = may be
+ * attended to), either or both NULL: keys outside them are not read, whatever they hold.  A row without any key gives
+ * zeros.  out [batch, queries, heads, dim] dense.  For a backward pass also out_f32 (the same, f32) and lse [batch, kv_heads,
+ * heads / kv_heads * queries] are written.
+ * The backward pass takes the forward call's arguments (out may be NULL), dout (strides like q's) and writes dq, dk, dv,
+ * dense; rows of dk / dv outside the masks are zeros.  kv heads shared by several query heads receive their sum. */
+typedef struct tapir_attn_args {
+  int64_t batch, queries, keys;
+  int heads, kv_heads, dim;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  void* out;
+  float *out_f32, *lse;
+  const void* dout;
+  int64_t dout_stride[3];
+  void *dq, *dk, *dv;
+  void* workspace;
+  uint64_t workspace_bytes;
+} tapir_attn_args;
+int tapir_cross_attention_workspace(tapir_ctx* ctx, const tapir_attn_args* args, int backward, uint64_t* bytes);
+int tapir_cross_attention(tapir_ctx* ctx, const tapir_attn_args* args, void* stream);
+int tapir_cross_attention_backward(tapir_ctx* ctx, const tapir_attn_args* args, void* stream);
+
 /* Kernel-level hooks for the micro-benchmarks (tools/kbench.py) and the tile-shape tests; no
  * reference counterpart.  One launch of the engine's MFMA GEMM  C = epi(A . W^T + bias):
  * A [M,lda], W [N,ldw] in the context's operand type (f32 or bf16 bits), bias [N] f32 or NULL;

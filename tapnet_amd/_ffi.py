@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_long, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_long, c_uint64, c_void_p
 
 TAPIR_OK = 0
 TAPIR_ERR_INVALID = -1
@@ -55,6 +55,24 @@ class TapirTrajArgs(ctypes.Structure):
               ('ctx1_in', c_void_p), ('ctx2_in', c_void_p),
               ('ctx1_out', c_void_p), ('ctx2_out', c_void_p),
               ('tracks', c_void_p), ('occlusion', c_void_p), ('expected_dist', c_void_p)]
+
+
+class TapirRotaryArgs(ctypes.Structure):   # tapir_rotary_args
+  _fields_ = [('batch', c_int64), ('tokens', c_int64),
+              ('heads', c_int), ('dim', c_int), ('axes', c_int), ('interleaved', c_int), ('inverse', c_int),
+              ('section', c_int * 4), ('base', c_double * 4), ('x', c_void_p), ('x_stride', c_int64 * 3),
+              ('positions', c_void_p), ('positions_stride', c_int64), ('y', c_void_p)]
+
+
+class TapirAttnArgs(ctypes.Structure):   # tapir_attn_args
+  _fields_ = [('batch', c_int64), ('queries', c_int64), ('keys', c_int64),
+              ('heads', c_int), ('kv_heads', c_int), ('dim', c_int), ('scale', c_float),
+              ('q', c_void_p), ('k', c_void_p), ('v', c_void_p),
+              ('q_stride', c_int64 * 3), ('k_stride', c_int64 * 3), ('v_stride', c_int64 * 3),
+              ('key_lengths', c_void_p), ('key_mask', c_void_p), ('out', c_void_p), ('out_f32', c_void_p),
+              ('lse', c_void_p), ('dout', c_void_p), ('dout_stride', c_int64 * 3),
+              ('dq', c_void_p), ('dk', c_void_p), ('dv', c_void_p), ('workspace', c_void_p),
+              ('workspace_bytes', c_uint64)]
 
 
 # name -> (restype, argtypes); every symbol include/tapir_hip.h declares
@@ -121,6 +139,15 @@ PROTOTYPES = {
     'tapir_conv_fused_dual_nn': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                          c_int, POINTER(TapirNextNorm), c_void_p]),
+    'tapir_layer_norm': (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                 c_float, c_void_p]),
+    'tapir_layer_norm_workspace': (c_int, [c_void_p, c_int64, c_int, POINTER(c_uint64)]),
+    'tapir_layer_norm_backward': (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_uint64, c_void_p]),
+    'tapir_rotary_positions': (c_int, [c_void_p, POINTER(TapirRotaryArgs), c_void_p]),
+    'tapir_cross_attention_workspace': (c_int, [c_void_p, POINTER(TapirAttnArgs), c_int, POINTER(c_uint64)]),
+    'tapir_cross_attention': (c_int, [c_void_p, POINTER(TapirAttnArgs), c_void_p]),
+    'tapir_cross_attention_backward': (c_int, [c_void_p, POINTER(TapirAttnArgs), c_void_p]),
     'tapir_debug_gemm': (c_int, [c_void_p, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p,
                                  c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int,
                                  c_void_p]),

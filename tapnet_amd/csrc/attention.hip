@@ -1,0 +1,341 @@
+// libtapir_hip: layer normalisation, rotary positions and cross attention -- argument checks, kernel choice and the C ABI
+// (include/tapir_hip.h).  A translation unit of its own: nothing here touches a context's weights or workspaces.
+#include "attention.hpp"
+
+#include <math.h>
+#include <stdio.h>
+
+#include <algorithm>
+
+#include "context.hpp"
+#include "layer_norm.hpp"
+#include "rotary.hpp"
+
+using namespace tapir;
+
+namespace {
+
+#define OP_TRY(c, expr)                                                                   \
+  do {                                                                                    \
+    const hipError_t e_ = (expr);                                                         \
+    if (e_ != hipSuccess) return ctx_fail((c), TAPIR_ERR_HIP, hipGetErrorString(e_));     \
+  } while (0)
+#define OP_REQUIRE(c, cond, code, msg)              \
+  do {                                              \
+    if (!(cond)) return ctx_fail((c), (code), msg); \
+  } while (0)
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// workgroups of a grid-stride launch: all that are resident at once (8 of 256 threads a CU), no more than there is work for
+unsigned stride_grid(long work, int per_cu = 8) { return (unsigned)std::max<long>(1, std::min<long>(work, 256L * per_cu)); }
+
+// ---------------------------------------------------------------------------------------------------- layer norm
+template <typename T, int EPT, int LPR, int NCH>
+void ln_launch(const LnArgs& a, hipStream_t s) {
+  const int rpb = LN_THREADS / LPR;
+  hipLaunchKernelGGL((layer_norm_kernel<T, EPT, LPR, NCH>), dim3(stride_grid((a.rows + rpb - 1) / rpb)), dim3(LN_THREADS), 0, s, a);
+}
+
+template <typename T, int EPT>
+void ln_dispatch(const LnArgs& a, hipStream_t s) {
+  const int chunks = (a.C + EPT - 1) / EPT;
+  if (chunks <= 8) ln_launch<T, EPT, 8, 1>(a, s);
+  else if (chunks <= 16) ln_launch<T, EPT, 16, 1>(a, s);
+  else if (chunks <= 32) ln_launch<T, EPT, 32, 1>(a, s);
+  else if (chunks <= 64) ln_launch<T, EPT, 64, 1>(a, s);
+  else if (chunks <= 128) ln_launch<T, EPT, 64, 2>(a, s);
+  else if (chunks <= 256) ln_launch<T, EPT, 64, 4>(a, s);
+  else if (EPT == 1 && chunks <= 1024) ln_launch<T, EPT, 64, EPT == 1 ? 16 : 4>(a, s);
+  else hipLaunchKernelGGL((layer_norm_long_kernel<T>), dim3(stride_grid(a.rows)), dim3(LN_THREADS), 0, s, a);
+}
+
+// rows a backward workgroup covers a step, and the workgroups (= shares of the parameters' gradients) of a launch
+int ln_bwd_rows(long chunks) { return chunks <= 8 ? 32 : chunks <= 16 ? 16 : chunks <= 32 ? 8 : 4; }
+
+int ln_ept(int dtype, int C, long ldx, const void* x, long ldy, const void* y, const void* z) {
+  const int v = dtype == TAPIR_BF16 ? 8 : 4;
+  return C % v == 0 && ldx % v == 0 && ldy % v == 0 && aligned16(x) && aligned16(y) && aligned16(z) ? v : 1;
+}
+
+// (C % 8 == 0 says nothing about alignment: the count below holds for both element widths of a launch)
+unsigned ln_bwd_grid(long rows, int C, int ept) {
+  const long chunks = (C + ept - 1) / ept;
+  const bool lng = chunks > (ept == 1 ? 1024 : 256);
+  const int rpb = lng ? 1 : ln_bwd_rows(chunks);
+  return stride_grid((rows + rpb - 1) / rpb, 2);
+}
+
+template <typename T, int EPT, int LPR, int NCH>
+void ln_bwd_launch(const LnBwdArgs& a, unsigned grid, hipStream_t s) {
+  hipLaunchKernelGGL((layer_norm_bwd_kernel<T, EPT, LPR, NCH>), dim3(grid), dim3(LN_THREADS), 0, s, a);
+}
+
+template <typename T, int EPT>
+void ln_bwd_dispatch(const LnBwdArgs& a, unsigned grid, hipStream_t s) {
+  const int chunks = (a.C + EPT - 1) / EPT;
+  if (chunks <= 8) ln_bwd_launch<T, EPT, 8, 1>(a, grid, s);
+  else if (chunks <= 16) ln_bwd_launch<T, EPT, 16, 1>(a, grid, s);
+  else if (chunks <= 32) ln_bwd_launch<T, EPT, 32, 1>(a, grid, s);
+  else if (chunks <= 64) ln_bwd_launch<T, EPT, 64, 1>(a, grid, s);
+  else if (chunks <= 128) ln_bwd_launch<T, EPT, 64, 2>(a, grid, s);
+  else if (chunks <= 256) ln_bwd_launch<T, EPT, 64, 4>(a, grid, s);
+  else if (EPT == 1 && chunks <= 1024) ln_bwd_launch<T, EPT, 64, EPT == 1 ? 16 : 4>(a, grid, s);
+  else hipLaunchKernelGGL((layer_norm_bwd_long_kernel<T>), dim3(grid), dim3(LN_THREADS), 0, s, a);
+}
+
+// ---------------------------------------------------------------------------------------------------- attention
+int attn_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+struct AttnPlan {
+  int dp, row_tiles, splits, tiles_per_split;
+  size_t part_o, part_ml;   // floats
+};
+
+// Key splits of the forward pass: where the row tiles alone leave compute units idle, the keys are cut until there are about
+// four workgroups a CU, each with four tiles at least (the join reads splits x rows partial results).
+AttnPlan attn_plan(const tapir_attn_args* a, int dtype) {
+  AttnPlan p{};
+  const int kt = dtype == TAPIR_BF16 ? 64 : 32;
+  p.dp = attn_pad(a->dim);
+  const long rows = (long)(a->heads / a->kv_heads) * a->queries;
+  p.row_tiles = (int)((rows + AT_QROWS - 1) / AT_QROWS);
+  const long tiles = std::max<long>(1, (a->keys + kt - 1) / kt);
+  const long base = std::max<long>(1, (long)a->batch * a->kv_heads * p.row_tiles);
+  long s = std::min<long>((1024 + base - 1) / base, (tiles + 3) / 4);
+  s = std::max<long>(1, std::min<long>(s, 1024));
+  p.tiles_per_split = (int)((tiles + s - 1) / s);
+  p.splits = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+  if (p.splits > 1) {
+    const size_t r = (size_t)p.splits * a->batch * a->kv_heads * rows;
+    p.part_o = r * p.dp;
+    p.part_ml = r * 2;
+  }
+  return p;
+}
+
+int attn_check(tapir_ctx* c, const tapir_attn_args* a, bool backward) {
+  OP_REQUIRE(c, a != nullptr, TAPIR_ERR_INVALID, "cross_attention: null arguments");
+  OP_REQUIRE(c, a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->heads >= 1 && a->kv_heads >= 1, TAPIR_ERR_INVALID,
+             "cross_attention: negative size or no heads");
+  OP_REQUIRE(c, a->heads % a->kv_heads == 0, TAPIR_ERR_INVALID, "cross_attention: heads is not a multiple of kv_heads");
+  OP_REQUIRE(c, a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0, TAPIR_ERR_UNSUPPORTED,
+             "cross_attention: head dimension has to be a multiple of 8, at most 128");
+  OP_REQUIRE(c, a->scale > 0.f && isfinite(a->scale), TAPIR_ERR_INVALID, "cross_attention: scale has to be positive and finite");
+  const long most = 1L << 30;   // rows, keys, and the workgroups of a launch stay below 2^31
+  OP_REQUIRE(c, a->queries <= most && a->keys <= most && (long)a->heads * a->queries <= most && (long)a->batch * a->heads <= (1 << 20),
+             TAPIR_ERR_UNSUPPORTED, "cross_attention: too many tokens or heads");
+  OP_REQUIRE(c, (long)a->batch * a->kv_heads * (((long)(a->heads / a->kv_heads) * a->queries + AT_QROWS - 1) / AT_QROWS) <= most &&
+                    (long)a->batch * a->kv_heads * ((a->keys + AT_KEYS - 1) / AT_KEYS) <= most,
+             TAPIR_ERR_UNSUPPORTED, "cross_attention: too many workgroups");
+  const int epc = ctx_info(c).dtype == TAPIR_BF16 ? 8 : 4;
+  auto tensor_ok = [&](const void* p, const int64_t* st, bool empty) {
+    return empty || (p && aligned16(p) && st[0] % epc == 0 && st[1] % epc == 0 && st[2] % epc == 0);
+  };
+  const bool no_q = a->batch == 0 || a->queries == 0, no_k = a->batch == 0 || a->keys == 0;
+  OP_REQUIRE(c, tensor_ok(a->q, a->q_stride, no_q) && tensor_ok(a->k, a->k_stride, no_k) && tensor_ok(a->v, a->v_stride, no_k) &&
+                    (!backward || tensor_ok(a->dout, a->dout_stride, no_q)),
+             TAPIR_ERR_INVALID, "cross_attention: null tensor, or one whose rows do not start at multiples of 16 bytes");
+  OP_REQUIRE(c, no_q || (a->out && aligned16(a->out)) || backward, TAPIR_ERR_INVALID, "cross_attention: null or misaligned output");
+  if (backward) {
+    OP_REQUIRE(c, no_q || (a->dq && aligned16(a->dq) && a->out_f32 && aligned16(a->out_f32) && a->lse), TAPIR_ERR_INVALID,
+               "cross_attention: the backward pass needs out_f32 and lse of the forward pass, and dq");
+    OP_REQUIRE(c, no_k || (a->dk && a->dv && aligned16(a->dk) && aligned16(a->dv)), TAPIR_ERR_INVALID,
+               "cross_attention: the backward pass needs dk and dv");
+  } else {
+    OP_REQUIRE(c, (a->out_f32 == nullptr) == (a->lse == nullptr) && aligned16(a->out_f32), TAPIR_ERR_INVALID,
+               "cross_attention: out_f32 and lse go together");
+  }
+  return TAPIR_OK;
+}
+
+AttnArgs attn_args(const tapir_attn_args* a, const AttnPlan& p) {
+  AttnArgs k{};
+  k.q = a->q; k.k = a->k; k.v = a->v; k.dout = a->dout;
+  for (int i = 0; i < 3; ++i) { k.qs[i] = a->q_stride[i]; k.ks[i] = a->k_stride[i]; k.vs[i] = a->v_stride[i]; k.ds[i] = a->dout_stride[i]; }
+  k.key_lengths = a->key_lengths; k.key_mask = a->key_mask;
+  k.out = a->out; k.out32 = a->out_f32; k.lse = a->lse; k.dq = a->dq; k.dk = a->dk; k.dv = a->dv;
+  k.B = a->batch; k.Hkv = a->kv_heads; k.G = a->heads / a->kv_heads; k.D = a->dim;
+  k.Nq = a->queries; k.Nk = a->keys; k.rows = (long)k.G * a->queries;
+  k.scale = a->scale; k.scale2 = a->scale * kLog2e;
+  k.splits = p.splits; k.tiles_per_split = p.tiles_per_split; k.row_tiles = p.row_tiles;
+  return k;
+}
+
+template <typename T, int DP>
+void attn_fwd_launch(const AttnArgs& k, hipStream_t s) {
+  const unsigned grid = (unsigned)((long)k.B * k.Hkv * k.row_tiles * k.splits);
+  hipLaunchKernelGGL((attn_fwd_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
+  if (k.splits > 1) {
+    const long rows = (long)k.B * k.Hkv * k.rows;
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k, DP);
+  }
+}
+
+template <typename T, int DP>
+void attn_bwd_launch(const AttnArgs& k, hipStream_t s) {
+  if (k.rows > 0) {
+    const unsigned grid = (unsigned)((long)k.B * k.Hkv * k.row_tiles);
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
+  }
+  if (k.Nk > 0) {
+    const unsigned grid = (unsigned)((long)k.B * k.Hkv * ((k.Nk + AT_KEYS - 1) / AT_KEYS));
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
+  }
+}
+
+#define ATTN_DISPATCH(fn, dtype, dp, ...)                                                                              \
+  do {                                                                                                                 \
+    if ((dtype) == TAPIR_BF16) {                                                                                       \
+      if ((dp) == 32) fn<bf16_t, 32>(__VA_ARGS__); else if ((dp) == 64) fn<bf16_t, 64>(__VA_ARGS__); else fn<bf16_t, 128>(__VA_ARGS__); \
+    } else {                                                                                                           \
+      if ((dp) == 32) fn<float, 32>(__VA_ARGS__); else if ((dp) == 64) fn<float, 64>(__VA_ARGS__); else fn<float, 128>(__VA_ARGS__);    \
+    }                                                                                                                  \
+  } while (0)
+
+size_t attn_backward_floats(const tapir_attn_args* a) { return (size_t)a->batch * a->heads * a->queries; }
+
+}  // namespace
+
+extern "C" {
+
+int tapir_layer_norm(tapir_ctx* c, const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y,
+                     float* mean, float* rstd, int64_t rows, int channels, float eps, void* stream) {
+  if (!c) return TAPIR_ERR_INVALID;
+  const CtxInfo ci = ctx_info(c);
+  OP_REQUIRE(c, rows >= 0 && channels >= 1 && eps >= 0.f && isfinite(eps), TAPIR_ERR_INVALID, "layer_norm: bad size or eps");
+  OP_REQUIRE(c, (mean == nullptr) == (rstd == nullptr), TAPIR_ERR_INVALID, "layer_norm: mean and rstd go together");
+  if (rows == 0) return TAPIR_OK;
+  OP_REQUIRE(c, x && y, TAPIR_ERR_INVALID, "layer_norm: null tensor");
+  OP_TRY(c, hipSetDevice(ci.device));
+  const LnArgs a{x, (long)x_stride, gamma, beta, y, mean, rstd, (long)rows, channels, eps};
+  const int ept = ln_ept(ci.dtype, channels, x_stride, x, channels, y, y);
+  hipStream_t s = (hipStream_t)stream;
+  if (ci.dtype == TAPIR_BF16) { if (ept == 8) ln_dispatch<bf16_t, 8>(a, s); else ln_dispatch<bf16_t, 1>(a, s); }
+  else { if (ept == 4) ln_dispatch<float, 4>(a, s); else ln_dispatch<float, 1>(a, s); }
+  OP_TRY(c, hipGetLastError());
+  return TAPIR_OK;
+}
+
+int tapir_layer_norm_workspace(tapir_ctx* c, int64_t rows, int channels, uint64_t* bytes) {
+  if (!c) return TAPIR_ERR_INVALID;
+  OP_REQUIRE(c, bytes && rows >= 0 && channels >= 1, TAPIR_ERR_INVALID, "layer_norm: bad size");
+  const int v = ctx_info(c).dtype == TAPIR_BF16 ? 8 : 4;
+  const unsigned shares = std::max(ln_bwd_grid(rows, channels, 1), ln_bwd_grid(rows, channels, v));
+  *bytes = (uint64_t)shares * 2 * channels * sizeof(float);
+  return TAPIR_OK;
+}
+
+int tapir_layer_norm_backward(tapir_ctx* c, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,
+                              const float* gamma, const float* mean, const float* rstd, void* dx, float* dgamma, float* dbeta,
+                              int64_t rows, int channels, void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (!c) return TAPIR_ERR_INVALID;
+  const CtxInfo ci = ctx_info(c);
+  OP_REQUIRE(c, rows >= 0 && channels >= 1, TAPIR_ERR_INVALID, "layer_norm: bad size");
+  OP_REQUIRE(c, rows == 0 || (x && dy && mean && rstd && dx), TAPIR_ERR_INVALID, "layer_norm: null tensor");
+  const int ept = ln_ept(ci.dtype, channels, x_stride, x, dy_stride, dy, dx);
+  const unsigned grid = ln_bwd_grid(rows, channels, ept);
+  const bool params = dgamma || dbeta;
+  OP_REQUIRE(c, !params || (workspace && aligned16(workspace) && workspace_bytes >= (uint64_t)grid * 2 * channels * sizeof(float)),
+             TAPIR_ERR_INVALID, "layer_norm: workspace missing or too small (tapir_layer_norm_workspace)");
+  OP_TRY(c, hipSetDevice(ci.device));
+  const LnBwdArgs a{x, (long)x_stride, dy, (long)dy_stride, gamma, mean, rstd, dx, params ? (float*)workspace : nullptr, (long)rows, channels};
+  hipStream_t s = (hipStream_t)stream;
+  if (rows > 0) {
+    if (ci.dtype == TAPIR_BF16) { if (ept == 8) ln_bwd_dispatch<bf16_t, 8>(a, grid, s); else ln_bwd_dispatch<bf16_t, 1>(a, grid, s); }
+    else { if (ept == 4) ln_bwd_dispatch<float, 4>(a, grid, s); else ln_bwd_dispatch<float, 1>(a, grid, s); }
+    OP_TRY(c, hipGetLastError());
+  }
+  if (params) {
+    hipLaunchKernelGGL(layer_norm_reduce_kernel, dim3((unsigned)((channels + LN_REDUCE_COLS - 1) / LN_REDUCE_COLS), 2), dim3(LN_THREADS), 0,
+                       s, (const float*)workspace, rows > 0 ? (int)grid : 0, channels, dgamma, dbeta);
+    OP_TRY(c, hipGetLastError());
+  }
+  return TAPIR_OK;
+}
+
+int tapir_rotary_positions(tapir_ctx* c, const tapir_rotary_args* r, void* stream) {
+  if (!c) return TAPIR_ERR_INVALID;
+  const CtxInfo ci = ctx_info(c);
+  OP_REQUIRE(c, r != nullptr, TAPIR_ERR_INVALID, "rotary_positions: null arguments");
+  OP_REQUIRE(c, r->batch >= 0 && r->tokens >= 0 && r->heads >= 1 && r->dim >= 1, TAPIR_ERR_INVALID, "rotary_positions: bad size");
+  OP_REQUIRE(c, r->dim <= 2 * ROT_MAX_PAIRS, TAPIR_ERR_UNSUPPORTED, "rotary_positions: head dimension over 256");
+  OP_REQUIRE(c, r->axes >= 1 && r->axes <= ROT_MAX_AXES, TAPIR_ERR_INVALID, "rotary_positions: 1 to 4 axes");
+  const long most = 1L << 40;
+  OP_REQUIRE(c, r->batch <= most && r->tokens <= most && (double)r->batch * r->tokens * r->heads * r->dim < 9e15, TAPIR_ERR_UNSUPPORTED,
+             "rotary_positions: too many tokens");
+  RotaryArgs a{};
+  int at = 0, pairs = 0;
+  for (int x = 0; x < r->axes; ++x) {
+    const int w = r->section[x];
+    OP_REQUIRE(c, w >= 0 && w % 2 == 0 && at + w <= r->dim, TAPIR_ERR_INVALID,
+               "rotary_positions: sections have to be even and fit the head dimension");
+    OP_REQUIRE(c, r->base[x] > 0.0 && isfinite(r->base[x]), TAPIR_ERR_INVALID, "rotary_positions: base has to be positive and finite");
+    for (int i = 0; i < w / 2; ++i, ++pairs) {
+      a.turns[pairs] = pow(r->base[x], -2.0 * i / w) / 6.283185307179586476925286766559;
+      a.axis[pairs] = (unsigned char)x;
+      a.lo[pairs] = (unsigned char)(r->interleaved ? at + 2 * i : at + i);
+      a.hi[pairs] = (unsigned char)(r->interleaved ? at + 2 * i + 1 : at + i + w / 2);
+    }
+    at += w;
+  }
+  if (r->batch == 0 || r->tokens == 0) return TAPIR_OK;
+  OP_REQUIRE(c, r->x && r->y && r->positions, TAPIR_ERR_INVALID, "rotary_positions: null tensor");
+  OP_TRY(c, hipSetDevice(ci.device));
+  a.x = r->x; a.sb = r->x_stride[0]; a.sn = r->x_stride[1]; a.sh = r->x_stride[2];
+  a.pos = r->positions; a.pb = r->positions_stride; a.y = r->y;
+  a.B = r->batch; a.N = r->tokens; a.H = r->heads; a.D = r->dim; a.axes = r->axes; a.pairs = pairs;
+  a.sign = r->inverse ? -1.f : 1.f;
+  const long work = (a.B * a.N * (a.D - a.pairs) + ROT_THREADS - 1) / ROT_THREADS;
+  const dim3 grid(stride_grid(work)), block(ROT_THREADS);
+  if (ci.dtype == TAPIR_BF16) hipLaunchKernelGGL((rotary_kernel<bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<float>), grid, block, 0, (hipStream_t)stream, a);
+  OP_TRY(c, hipGetLastError());
+  return TAPIR_OK;
+}
+
+int tapir_cross_attention_workspace(tapir_ctx* c, const tapir_attn_args* a, int backward, uint64_t* bytes) {
+  if (!c) return TAPIR_ERR_INVALID;
+  OP_REQUIRE(c, a && bytes && a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->kv_heads >= 1 && a->heads >= 1 &&
+                    a->heads % a->kv_heads == 0, TAPIR_ERR_INVALID, "cross_attention: bad size");
+  const AttnPlan p = attn_plan(a, ctx_info(c).dtype);
+  *bytes = sizeof(float) * (backward ? attn_backward_floats(a) : p.part_o + p.part_ml);
+  return TAPIR_OK;
+}
+
+int tapir_cross_attention(tapir_ctx* c, const tapir_attn_args* a, void* stream) {
+  if (!c) return TAPIR_ERR_INVALID;
+  const CtxInfo ci = ctx_info(c);
+  const int rc = attn_check(c, a, false);
+  if (rc != TAPIR_OK) return rc;
+  if (a->batch == 0 || a->queries == 0) return TAPIR_OK;
+  const AttnPlan p = attn_plan(a, ci.dtype);
+  OP_REQUIRE(c, p.splits == 1 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= sizeof(float) * (p.part_o + p.part_ml)),
+             TAPIR_ERR_INVALID, "cross_attention: workspace missing or too small (tapir_cross_attention_workspace)");
+  OP_TRY(c, hipSetDevice(ci.device));
+  AttnArgs k = attn_args(a, p);
+  k.part_o = (float*)a->workspace;
+  k.part_ml = (float*)a->workspace + p.part_o;
+  ATTN_DISPATCH(attn_fwd_launch, ci.dtype, p.dp, k, (hipStream_t)stream);
+  OP_TRY(c, hipGetLastError());
+  return TAPIR_OK;
+}
+
+int tapir_cross_attention_backward(tapir_ctx* c, const tapir_attn_args* a, void* stream) {
+  if (!c) return TAPIR_ERR_INVALID;
+  const CtxInfo ci = ctx_info(c);
+  const int rc = attn_check(c, a, true);
+  if (rc != TAPIR_OK) return rc;
+  if (a->batch == 0) return TAPIR_OK;
+  OP_REQUIRE(c, a->queries == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= sizeof(float) * attn_backward_floats(a)),
+             TAPIR_ERR_INVALID, "cross_attention: workspace missing or too small (tapir_cross_attention_workspace)");
+  OP_TRY(c, hipSetDevice(ci.device));
+  const AttnPlan p = attn_plan(a, ci.dtype);
+  AttnArgs k = attn_args(a, p);
+  k.delta = (float*)a->workspace;
+  ATTN_DISPATCH(attn_bwd_launch, ci.dtype, p.dp, k, (hipStream_t)stream);
+  OP_TRY(c, hipGetLastError());
+  return TAPIR_OK;
+}
+
+}  // extern "C"

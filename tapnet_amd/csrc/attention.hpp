@@ -1,0 +1,539 @@
+// Cross attention of query rows to an encoder's tokens, forward and backward, one pass over the keys.
+//
+//   s_rk = scale q_r . k_k,  p_rk = exp(s_rk - L_r),  L_r = log sum_k exp(s_rk),  o_r = sum_k p_rk v_k
+//   D_r = do_r . o_r,  dp_rk = do_r . v_k,  ds_rk = p_rk (dp_rk - D_r) scale
+//   dq_r = sum_k ds_rk k_k,   dk_k = sum_r ds_rk q_r,   dv_k = sum_r p_rk do_r
+//
+// Rows: the G query heads that share a key head are flattened with the queries into one row axis (row = g * queries + query),
+// so that a tile of rows reads every key once for all heads of the group, and the sums dk / dv of a shared head need no
+// reduction of their own.  Masked keys (behind the clip's length, or cleared in the key mask) are never loaded: their rows of
+// the tile are zeros and their scores -inf, so whatever the padding holds (NaN, infinities) cannot reach a result.  A row
+// without any key gives zeros and passes zero gradients.
+//
+// Matrix products: v_mfma_f32_32x32x16_bf16 / v_mfma_f32_32x32x2_f32.  The forward pass and dq work on TRANSPOSED scores
+// (rows of the product = keys, columns = query rows): a lane then holds 16 keys of ONE query row, the softmax statistics are
+// per-lane scalars (one exchange with lane ^ 32), and the 8 probabilities a lane holds in consecutive registers ARE its operand
+// of the next product (the order of the summed keys is free as long as both operands agree): nothing is moved between the
+// products.  dk / dv use the untransposed scores for the same reason (a lane holds 16 query rows of one key).  The other
+// operand of these second products is a transposed tile: ds_read_b64_tr_b16 (bf16), plain 4-byte reads (f32).
+#pragma once
+#include "common.hpp"
+
+namespace tapir {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+
+constexpr int AT_WAVES = 4;
+constexpr int AT_THREADS = 64 * AT_WAVES;
+constexpr int AT_QROWS = 32 * AT_WAVES;      // query rows of a forward / dq workgroup
+constexpr int AT_KEYS = 32 * AT_WAVES;       // keys of a dk / dv workgroup
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+  const void *q, *k, *v, *dout;
+  long qs[3], ks[3], vs[3], ds[3];     // strides in elements: clip, token, head (channels dense)
+  const int* key_lengths;              // [B] or null
+  const unsigned char* key_mask;       // [B, Nk] or null: nonzero = may be attended to
+  void* out;                           // [B, Nq, H, D] dense
+  float *out32;                        // the same unrounded (training), or null
+  float *lse;                          // [B, Hkv, G * Nq]: L_r in powers of two (0 for a row without keys), or null
+  float *delta;                        // [B, Hkv, G * Nq]: D_r
+  void *dq, *dk, *dv;                  // dense
+  float *part_o, *part_ml;             // split keys: [splits, B * Hkv, rows, DP] and [splits, B * Hkv, rows, 2]
+  long Nq, Nk, rows;                   // rows = G * Nq
+  int B, Hkv, G, D;
+  int splits, tiles_per_split;         // key tiles of a split
+  int row_tiles;
+  float scale, scale2;                 // scale, scale * log2(e)
+};
+
+__device__ __attribute__((aligned(16))) const unsigned at_zero16[4] = {0u, 0u, 0u, 0u};
+
+// physical 16-byte chunk of logical chunk c in row r of a tile with CH chunks a row: eight consecutive rows reading the same
+// chunk, and four consecutive rows reading a pair of chunks, each touch all banks once.
+template <int CH> __device__ __forceinline__ int at_swizzle(int r, int c) {
+  if (CH >= 8) return c ^ (((r & 3) << 1) | ((r >> 2) & 1));
+  return c ^ ((r & 2) | ((r >> 2) & 1));        // 64-byte rows: the row's parity picks the half of a bank line already
+}
+
+template <typename T> struct AtFrag;            // 16 bytes of a row: the operand of one k-step
+template <> struct AtFrag<bf16_t> { static constexpr int EPC = 8; };
+template <> struct AtFrag<float> { static constexpr int EPC = 4; };
+
+// c += a b over the elements of one 16-byte chunk per lane (lanes l and l ^ 32 hold neighbouring chunks)
+__device__ __forceinline__ f32x16 at_mma(const uint4& a, const uint4& b, f32x16 c, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 at_mma(const uint4& a, const uint4& b, f32x16 c, float) {
+  c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+}
+
+// ds_read_b64_tr_b16: the 16 lanes of a group name 16 x 8 bytes (lane i: row i / 4, columns 4 (i % 4) .. +3 of a 4 x 16 block);
+// lane i receives column i of the block, rows 0 .. 3.
+__device__ __forceinline__ uint2 at_read_tr(const bf16_t* p) {
+#ifdef TAPIR_HIPEMU
+  const unsigned l = threadIdx.x & 63, i = l & 15;
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  uint16_t r[4];
+  for (int j = 0; j < 4; ++j) {
+    const int src = (int)((l & 48) + 4 * j + (i >> 2));
+    const uint64_t hi = (uint32_t)__shfl((int)(a >> 32), src), lo = (uint32_t)__shfl((int)a, src);
+    r[j] = ((const uint16_t*)(uintptr_t)((hi << 32) | lo))[i & 3];
+  }
+  return make_uint2((unsigned)r[0] | ((unsigned)r[1] << 16), (unsigned)r[2] | ((unsigned)r[3] << 16));
+#else
+  typedef __attribute__((ext_vector_type(4))) short s16x4;
+  typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(uintptr_t)p);
+  return __builtin_bit_cast(uint2, r);
+#endif
+}
+
+// c[32 channels from d0][32 columns] += X[32 summed rows from r0][channels]^T * w, w = 16 values a lane in the layout of a
+// 32 x 32 product (register i of lane half h: summed row 8 (i / 4) + 4 h + i % 4).  X: a tile of CH-chunk rows in LDS.
+template <int CH>
+__device__ __forceinline__ void at_mma_tr(f32x16& c, const bf16_t* X, int r0, int d0, const unsigned (&w)[8]) {
+  const int l = threadIdx.x & 63, h = l >> 5, i = l & 15;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    uint2 t[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = r0 + 16 * s + 8 * u + 4 * h + (i >> 2), col = d0 + (l & 16) + 4 * (i & 3);
+      t[u] = at_read_tr(X + ((long)r * CH + at_swizzle<CH>(r, col >> 3)) * 8 + (col & 7));
+    }
+    c = at_mma(make_uint4(t[0].x, t[0].y, t[1].x, t[1].y), make_uint4(w[4 * s], w[4 * s + 1], w[4 * s + 2], w[4 * s + 3]), c, bf16_t{});
+  }
+}
+template <int CH>
+__device__ __forceinline__ void at_mma_tr(f32x16& c, const float* X, int r0, int d0, const float (&w)[16]) {
+  const int l = threadIdx.x & 63, h = l >> 5, col = d0 + (l & 31);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + 8 * (i >> 2) + 4 * h + (i & 3);
+    const float x = X[((long)r * CH + at_swizzle<CH>(r, col >> 2)) * 4 + (col & 3)];
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x, w[i], c, 0, 0, 0);
+  }
+}
+
+// the 16 values of a lane as the operand of at_mma_tr: rounded to bf16 (the products of the next sum take bf16 operands; the
+// relative error 2^-9 of each term is the size of the output's own rounding and averages out over the sum), or as they are
+__device__ __forceinline__ void at_operand(const f32x16& p, unsigned (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+}
+__device__ __forceinline__ void at_operand(const f32x16& p, float (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = p[i];
+}
+template <typename T> struct AtOperand;
+template <> struct AtOperand<bf16_t> { unsigned w[8]; };
+template <> struct AtOperand<float> { float w[16]; };
+
+__device__ __forceinline__ f32x16 at_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// ROWS x DP tile of a [token][channel] tensor -> LDS, 16-byte chunks, by the whole workgroup.  Row r of the tile is token
+// tok(r) (its address from `at`), or zeros where at() gives null; channels from D on are zeros too.
+template <typename T, int ROWS, int DP, class At>
+__device__ __forceinline__ void at_stage(T* lds, int D, const At& at) {
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, N = ROWS * CH / AT_THREADS;
+  static_assert(ROWS * CH % AT_THREADS == 0, "tile");
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int slot = n * AT_THREADS + (int)threadIdx.x;
+    const int r = slot / CH, c = at_swizzle<CH>(r, slot % CH);
+    const T* p = at(r);
+    const void* src = p != nullptr && c * EPC < D ? (const void*)(p + c * EPC) : (const void*)at_zero16;
+    glds16(src, lds + (long)(n * AT_THREADS + wave * 64) * EPC);
+  }
+}
+
+template <typename T, int CH> __device__ __forceinline__ uint4 at_chunk(const T* X, int r, int c) {
+  return *reinterpret_cast<const uint4*>(X + ((long)r * CH + at_swizzle<CH>(r, c)) * AtFrag<T>::EPC);
+}
+
+// key validity of the 64 keys from k0 as a wave-uniform mask (bit j: key k0 + j takes part)
+__device__ __forceinline__ uint64_t at_key_bits(const AttnArgs& a, int b, long k0, long len) {
+  const long key = k0 + (threadIdx.x & 63);
+  bool ok = key < len;
+  if (a.key_mask != nullptr && ok) ok = a.key_mask[(long)b * a.Nk + key] != 0;
+  return __ballot(ok);
+}
+
+__device__ __forceinline__ long at_key_len(const AttnArgs& a, int b) {
+  if (a.key_lengths == nullptr) return a.Nk;
+  const long n = a.key_lengths[b];
+  return n < 0 ? 0 : (n > a.Nk ? a.Nk : n);
+}
+
+// 4 consecutive channels of a result row
+template <typename T> __device__ __forceinline__ void at_store4(T* p, float x, float y, float z, float w);
+template <> __device__ __forceinline__ void at_store4<float>(float* p, float x, float y, float z, float w) {
+  *reinterpret_cast<float4*>(p) = make_float4(x, y, z, w);
+}
+template <> __device__ __forceinline__ void at_store4<bf16_t>(bf16_t* p, float x, float y, float z, float w) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x, y), pack_bf16x2(z, w));
+}
+
+// XCD-aware order: workgroups are dealt to the 8 dies in turn; consecutive WORK indices (row tiles of one key range) get the
+// same die, whose L2 then serves the keys to all of them.
+__device__ __forceinline__ long at_work_index() {
+  const long n = gridDim.x, i = blockIdx.x, per = n / 8, rem = n % 8, x = i % 8, j = i / 8;
+  return x * per + (x < rem ? x : rem) + j;
+}
+
+// keys a forward / dq step stages: 64 (bf16) or 32 (f32)
+template <typename T> struct AtTile { static constexpr int KT = sizeof(T) == 2 ? 64 : 32; };
+// query rows a dk / dv step stages: 32, or 64 where 32 rows are less than a copy per thread
+template <typename T, int DP> struct AtRowTile { static constexpr int RT = 32 * DP * (int)sizeof(T) / 16 >= AT_THREADS ? 32 : 64; };
+
+// ---------------------------------------------------------------------------------------------------------------- forward
+// A workgroup: AT_QROWS query rows of one key head, `tiles_per_split` key tiles; two LDS buffers, the next tile's copies in
+// flight under the current tile's products.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
+  __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
+  long w = at_work_index();
+  const int rt = (int)(w % a.row_tiles); w /= a.row_tiles;
+  const int split = (int)(w % a.splits); w /= a.splits;
+  const int hk = (int)(w % a.Hkv), b = (int)(w / a.Hkv);
+  const long row = (long)rt * AT_QROWS + wave * 32 + (l & 31);
+  const bool live = row < a.rows;
+  const long rr = live ? row : 0;
+  const int head = hk * a.G + (int)(rr / a.Nq);
+  const long query = rr % a.Nq;
+  const long len = at_key_len(a, b);
+  const int t0 = split * a.tiles_per_split;
+  const long n_tiles = (len + KT - 1) / KT;
+  const int t1 = (int)(n_tiles < (long)t0 + a.tiles_per_split ? n_tiles : (long)t0 + a.tiles_per_split);
+  const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+
+  uint4 qf[CH / 2];
+  const T* qp = (const T*)a.q + b * a.qs[0] + query * a.qs[1] + head * a.qs[2];
+#pragma unroll
+  for (int s = 0; s < CH / 2; ++s) {
+    const int c = 2 * s + h;
+    qf[s] = live && c * EPC < a.D ? ldg16(qp + c * EPC) : make_uint4(0, 0, 0, 0);
+  }
+  f32x16 o[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) o[d] = at_zero();
+  float m = -INFINITY, sum = 0.f;
+
+  uint64_t bits = 0;
+  auto stage = [&](int t, int buf) {
+    const long k0 = (long)t * KT;
+    bits = at_key_bits(a, b, k0, len);
+    at_stage<T, KT, DP>(kt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? kp + (k0 + r) * a.ks[1] : (const T*)nullptr; });
+    at_stage<T, KT, DP>(vt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? vp + (k0 + r) * a.vs[1] : (const T*)nullptr; });
+  };
+  if (t0 < t1) stage(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const uint64_t cur = bits;
+    dma_wait<0>();
+    __syncthreads();
+    if (t + 1 < t1) stage(t + 1, buf ^ 1);
+    f32x16 s[KT / 32];
+    float top = m;
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      s[kb] = at_zero();
+#pragma unroll
+      for (int x = 0; x < CH / 2; ++x) s[kb] = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s[kb], T{});
+      const unsigned mb = (unsigned)(cur >> (32 * kb));
+      if (mb != 0xffffffffu) {
+        const unsigned mine = mb >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[kb][i] : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float base = top == -INFINITY ? 0.f : top * a.scale2;
+    const float alpha = fast_exp2(fmaf(m, a.scale2, -base));
+    m = top;
+    sum *= alpha;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -base));
+        sum += s[kb][i];
+      }
+      AtOperand<T> p;
+      at_operand(s[kb], p.w);
+#pragma unroll
+      for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], vt[buf], kb * 32, d * 32, p.w);
+    }
+  }
+  sum += __shfl_xor(sum, 32);
+  if (!live) return;
+  const long bh = (long)b * a.Hkv + hk;
+  if (a.splits > 1) {
+    const long at = ((long)split * a.B * a.Hkv + bh) * a.rows + row;
+    float* po = a.part_o + at * DP;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        at_store4<float>(po + d * 32 + 8 * i + 4 * h, o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m == -INFINITY ? m : m * a.scale2, sum);
+    return;
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const long at = (((long)b * a.Nq + query) * a.Hkv * a.G + head) * a.D;
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = d * 32 + 8 * i + 4 * h;
+      if (c < a.D) {
+        const float x = o[d][4 * i] * inv, y = o[d][4 * i + 1] * inv, z = o[d][4 * i + 2] * inv, u = o[d][4 * i + 3] * inv;
+        at_store4<T>((T*)a.out + at + c, x, y, z, u);
+        if (a.out32) at_store4<float>(a.out32 + at + c, x, y, z, u);
+      }
+    }
+  if (a.lse && h == 0) a.lse[bh * a.rows + row] = sum > 0.f ? fmaf(m, a.scale2, log2f(sum)) : 0.f;
+}
+
+// joins the key splits: a wave a row;  o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s
+template <typename T>
+__global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a, int DP) {
+  const long bhs = (long)a.B * a.Hkv, total = bhs * a.rows;
+  const int l = threadIdx.x & 63;
+  const long r = (long)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
+  if (r >= total) return;
+  float top = -INFINITY;
+  for (int s = l; s < a.splits; s += 64) top = fmaxf(top, a.part_ml[2 * (s * total + r)]);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int s = l; s < a.splits; s += 64) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * total + r));
+    sum = fmaf(fast_exp2(ml.x - base), ml.y, sum);
+  }
+  sum = wave_sum(sum);
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const long bh = r / a.rows, row = r % a.rows, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const long at = ((b * a.Nq + row % a.Nq) * a.Hkv * a.G + hk * a.G + row / a.Nq) * a.D;
+  for (int c = l; c < a.D; c += 64) {
+    float x = 0.f;
+    for (int s = 0; s < a.splits; ++s)
+      x = fmaf(fast_exp2(a.part_ml[2 * (s * total + r)] - base), a.part_o[(s * total + r) * DP + c], x);
+    x *= inv;
+    Elem<T>::st((T*)a.out + at + c, x);
+    if (a.out32) a.out32[at + c] = x;
+  }
+  if (a.lse && l == 0) a.lse[r] = sum > 0.f ? base + log2f(sum) : 0.f;
+}
+
+// --------------------------------------------------------------------------------------------------------------- backward
+// dq (and D_r on the way): the forward kernel's loop with p from the saved L_r.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
+  __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
+  long w = at_work_index();
+  const int rt = (int)(w % a.row_tiles); w /= a.row_tiles;
+  const int hk = (int)(w % a.Hkv), b = (int)(w / a.Hkv);
+  const long row = (long)rt * AT_QROWS + wave * 32 + (l & 31);
+  const bool live = row < a.rows;
+  const long rr = live ? row : 0;
+  const int head = hk * a.G + (int)(rr / a.Nq);
+  const long query = rr % a.Nq;
+  const long len = at_key_len(a, b);
+  const int n_tiles = (int)((len + KT - 1) / KT);
+  const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+  const long bh = (long)b * a.Hkv + hk;
+  const long at = (((long)b * a.Nq + query) * a.Hkv * a.G + head) * a.D;
+
+  uint4 qf[CH / 2], gf[CH / 2];
+  const T* qp = (const T*)a.q + b * a.qs[0] + query * a.qs[1] + head * a.qs[2];
+  const T* gp = (const T*)a.dout + b * a.ds[0] + query * a.ds[1] + head * a.ds[2];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < CH / 2; ++s) {
+    const int c = 2 * s + h;
+    const bool in = live && c * EPC < a.D;
+    qf[s] = in ? ldg16(qp + c * EPC) : make_uint4(0, 0, 0, 0);
+    gf[s] = in ? ldg16(gp + c * EPC) : make_uint4(0, 0, 0, 0);
+    if (in) {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) delta = fmaf(Elem<T>::ld(gp + c * EPC + e), a.out32[at + c * EPC + e], delta);
+    }
+  }
+  delta += __shfl_xor(delta, 32);
+  const float lse = a.lse[bh * a.rows + rr];
+  if (live && h == 0) a.delta[bh * a.rows + row] = delta;
+  f32x16 o[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) o[d] = at_zero();
+
+  uint64_t bits = 0;
+  auto stage = [&](int t, int buf) {
+    const long k0 = (long)t * KT;
+    bits = at_key_bits(a, b, k0, len);
+    at_stage<T, KT, DP>(kt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? kp + (k0 + r) * a.ks[1] : (const T*)nullptr; });
+    at_stage<T, KT, DP>(vt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? vp + (k0 + r) * a.vs[1] : (const T*)nullptr; });
+  };
+  if (n_tiles > 0) stage(0, 0);
+  for (int t = 0; t < n_tiles; ++t) {
+    const int buf = t & 1;
+    const uint64_t cur = bits;
+    dma_wait<0>();
+    __syncthreads();
+    if (t + 1 < n_tiles) stage(t + 1, buf ^ 1);
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      f32x16 s = at_zero(), g = at_zero();
+#pragma unroll
+      for (int x = 0; x < CH / 2; ++x) {
+        s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
+        g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
+      }
+      const unsigned mine = (unsigned)(cur >> (32 * kb)) >> (4 * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = fast_exp2(fmaf(s[i], a.scale2, -lse)) * (g[i] - delta);
+        s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? p : 0.f;
+      }
+      AtOperand<T> p;
+      at_operand(s, p.w);
+#pragma unroll
+      for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], kt[buf], kb * 32, d * 32, p.w);
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = d * 32 + 8 * i + 4 * h;
+      if (c < a.D)
+        at_store4<T>((T*)a.dq + at + c, o[d][4 * i] * a.scale, o[d][4 * i + 1] * a.scale, o[d][4 * i + 2] * a.scale,
+                     o[d][4 * i + 3] * a.scale);
+    }
+}
+
+// dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads, RT at a time.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
+  __shared__ __attribute__((aligned(16))) T qt[2][RT * DP];
+  __shared__ __attribute__((aligned(16))) T gt[2][RT * DP];
+  __shared__ __attribute__((aligned(16))) float ld[2][2][RT];   // L_r, D_r
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
+  const long key_tiles = (a.Nk + AT_KEYS - 1) / AT_KEYS;
+  long w = at_work_index();
+  const long kt = w % key_tiles; w /= key_tiles;
+  const int hk = (int)(w % a.Hkv), b = (int)(w / a.Hkv);
+  const long key = kt * AT_KEYS + wave * 32 + (l & 31);
+  const long len = at_key_len(a, b);
+  bool in = key < len;
+  if (in && a.key_mask != nullptr) in = a.key_mask[(long)b * a.Nk + key] != 0;
+  const long bh = (long)b * a.Hkv + hk;
+  uint4 kf[CH / 2], vf[CH / 2];
+  const T* kp = (const T*)a.k + b * a.ks[0] + (in ? key : 0) * a.ks[1] + hk * a.ks[2];
+  const T* vp = (const T*)a.v + b * a.vs[0] + (in ? key : 0) * a.vs[1] + hk * a.vs[2];
+#pragma unroll
+  for (int s = 0; s < CH / 2; ++s) {
+    const int c = 2 * s + h;
+    kf[s] = in && c * EPC < a.D ? ldg16(kp + c * EPC) : make_uint4(0, 0, 0, 0);
+    vf[s] = in && c * EPC < a.D ? ldg16(vp + c * EPC) : make_uint4(0, 0, 0, 0);
+  }
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) { dk[d] = at_zero(); dv[d] = at_zero(); }
+  // (a tile behind the clip's length has nothing to add: no steps, zeros are stored)
+  const int n_tiles = kt * AT_KEYS < len ? (int)((a.rows + RT - 1) / RT) : 0;
+  auto stage = [&](int t, int buf) {
+    const long r0 = (long)t * RT;
+    at_stage<T, RT, DP>(qt[buf], a.D, [&](int r) {
+      const long row = r0 + r;
+      return row < a.rows ? (const T*)a.q + b * a.qs[0] + (row % a.Nq) * a.qs[1] + (hk * a.G + row / a.Nq) * a.qs[2] : (const T*)nullptr;
+    });
+    at_stage<T, RT, DP>(gt[buf], a.D, [&](int r) {
+      const long row = r0 + r;
+      return row < a.rows ? (const T*)a.dout + b * a.ds[0] + (row % a.Nq) * a.ds[1] + (hk * a.G + row / a.Nq) * a.ds[2] : (const T*)nullptr;
+    });
+    if (threadIdx.x < 2 * RT) {
+      const long row = r0 + (threadIdx.x & (RT - 1));
+      const float* src = threadIdx.x < RT ? a.lse : a.delta;
+      ld[buf][threadIdx.x / RT][threadIdx.x & (RT - 1)] = row < a.rows ? src[bh * a.rows + row] : 0.f;
+    }
+  };
+  if (n_tiles > 0) stage(0, 0);
+  for (int t = 0; t < n_tiles; ++t) {
+    const int buf = t & 1;
+    dma_wait<0>();
+    __syncthreads();
+    if (t + 1 < n_tiles) stage(t + 1, buf ^ 1);
+#pragma unroll
+    for (int rb = 0; rb < RT; rb += 32) {
+      f32x16 s = at_zero(), g = at_zero();
+#pragma unroll
+      for (int x = 0; x < CH / 2; ++x) {
+        s = at_mma(at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
+        g = at_mma(at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 L = *reinterpret_cast<const float4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
+        const float4 E = *reinterpret_cast<const float4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
+        const float Lv[4] = {L.x, L.y, L.z, L.w}, Ev[4] = {E.x, E.y, E.z, E.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = in ? fast_exp2(fmaf(s[4 * i + j], a.scale2, -Lv[j])) : 0.f;
+          s[4 * i + j] = p;
+          g[4 * i + j] = p * (g[4 * i + j] - Ev[j]);
+        }
+      }
+      AtOperand<T> p, e;
+      at_operand(s, p.w);
+      at_operand(g, e.w);
+#pragma unroll
+      for (int d = 0; d < NB; ++d) {
+        at_mma_tr<CH>(dv[d], gt[buf], rb, d * 32, p.w);
+        at_mma_tr<CH>(dk[d], qt[buf], rb, d * 32, e.w);
+      }
+    }
+  }
+  if (key >= a.Nk) return;
+  const long at = (((long)b * a.Nk + key) * a.Hkv + hk) * a.D;
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = d * 32 + 8 * i + 4 * h;
+      if (c < a.D) {
+        at_store4<T>((T*)a.dk + at + c, dk[d][4 * i] * a.scale, dk[d][4 * i + 1] * a.scale, dk[d][4 * i + 2] * a.scale,
+                     dk[d][4 * i + 3] * a.scale);
+        at_store4<T>((T*)a.dv + at + c, dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]);
+      }
+    }
+}
+
+}  // namespace tapir

@@ -13,6 +13,7 @@
 
 #include "backbone.hpp"
 #include "common.hpp"
+#include "context.hpp"
 #include "conv_fused.hpp"
 #include "conv_flat.hpp"
 #include "conv_small.hpp"
@@ -1252,6 +1253,20 @@ int do_estimate(tapir_ctx* c, const tapir_traj_args* a, hipStream_t s) {
 }
 
 }  // namespace
+
+namespace tapir {
+
+CtxInfo ctx_info(const tapir_ctx* c) { return CtxInfo{c->device, c->cfg.dtype, c->n_cus}; }
+
+int ctx_fail(tapir_ctx* c, int code, const char* msg) noexcept {
+  try {
+    if (c) c->err = msg;
+  } catch (...) {   // (out of memory: the code still says what kind of error it was)
+  }
+  return code;
+}
+
+}  // namespace tapir
 
 // ============================================================================
 // C ABI

@@ -14,5 +14,16 @@ if [ "$1" == "--asan" ]; then
   OUT=libtapir_emu_asan.so
   SAN="-fsanitize=address,undefined -fno-sanitize=vptr,function -fno-omit-frame-pointer -shared-libsan -g1"
 fi
-/opt/rocm/lib/llvm/bin/clang++ -x c++ -std=c++17 -O2 -fopenmp -fPIC -shared -I. -DTAPIR_EXPERIMENTS $SAN \
-  -Wno-unused-value ../../tapnet_amd/csrc/engine.hip emu_switch.cpp -o $OUT "$@"
+# one object per translation unit, compiled side by side (build_emu.sh --unit attention: that one only, then the link)
+CXX=/opt/rocm/lib/llvm/bin/clang++
+OBJ=build/${OUT%.so}
+mkdir -p "$OBJ"
+UNITS="engine attention"
+if [ "$1" == "--unit" ]; then UNITS=$2; shift 2; fi
+PIDS=""
+for u in $UNITS; do
+  $CXX -x c++ -std=c++17 -O2 -fopenmp -fPIC -I. -DTAPIR_EXPERIMENTS $SAN -Wno-unused-value -c ../../tapnet_amd/csrc/$u.hip -o "$OBJ/$u.o" "$@" &
+  PIDS="$PIDS $!"
+done
+for p in $PIDS; do wait $p; done
+$CXX -std=c++17 -O2 -fopenmp -fPIC -shared -I. $SAN "$OBJ/engine.o" "$OBJ/attention.o" -x c++ emu_switch.cpp -o $OUT "$@"

@@ -412,6 +412,18 @@ template <class T> static inline T __shfl_up(T v, unsigned d, int width = 64) {
   if (src < 0 || (src & ~(width - 1)) != (lane & ~(width - 1))) src = lane;
   return hipemu_shfl_idx(v, src);
 }
+static inline uint64_t __ballot(int pred) {
+  uint64_t out = 0;
+  hipemu::wave_collective(
+      [&](hipemu::WaveBuf& wb, unsigned lane) { wb.v[lane][0] = pred != 0; wb.v[lane][1] = 1; },
+      [&](hipemu::WaveBuf& wb) {
+        uint64_t m = 0;
+        for (int l = 0; l < 64; ++l) { if (wb.v[l][1] && wb.v[l][0]) m |= 1ull << l; wb.v[l][1] = 0; }
+        memcpy(&wb.v[0][2], &m, 8);
+      },
+      [&](hipemu::WaveBuf& wb, unsigned lane) { (void)lane; memcpy(&out, &wb.v[0][2], 8); });
+  return out;
+}
 static inline int __builtin_amdgcn_readfirstlane(int v) { return hipemu_shfl_idx(v, 0); }
 
 // ---------------------------------------------------------------- MFMA
