@@ -408,7 +408,7 @@ int tapir_xconv_nt(tapir_ctx* ctx, const void* x, const void* wstream, const flo
  * addresses are read and written 16 bytes at a time. */
 int tapir_layer_norm(tapir_ctx* ctx, const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y,
                      float* mean, float* rstd, int64_t rows, int channels, float eps, void* stream);
-/* dx (dense), dgamma, dbeta [channels] (either may be NULL; they are overwritten, not added to). */
+/* dx (dense), dgamma, dbeta [channels]: any of them may be NULL; they are overwritten, not added to. */
 int tapir_layer_norm_workspace(tapir_ctx* ctx, int64_t rows, int channels, uint64_t* bytes);
 int tapir_layer_norm_backward(tapir_ctx* ctx, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,
                               const float* gamma, const float* mean, const float* rstd, void* dx, float* dgamma,
@@ -439,10 +439,11 @@ int tapir_rotary_positions(tapir_ctx* ctx, const tapir_rotary_args* args, void* 
  * token, head) in elements, channels dense, every row at a multiple of 16 bytes; dim a multiple of 8, at most 128;
  * scale > 0.  key_lengths [batch] int32 (device; clamped to 0 .. keys) and key_mask [batch, keys] bytes (nonzero = may be
  * attended to), either or both NULL: keys outside them are not read, whatever they hold.  A row without any key gives
- * zeros.  out [batch, queries, heads, dim] dense.  For a backward pass also out_f32 (the same, f32) and lse [batch, kv_heads,
- * heads / kv_heads * queries] are written.
- * The backward pass takes the forward call's arguments (out may be NULL), dout (strides like q's) and writes dq, dk, dv,
- * dense; rows of dk / dv outside the masks are zeros.  kv heads shared by several query heads receive their sum. */
+ * zeros.  out [batch, queries, heads, dim] dense.  For a backward pass also out_f32 (the same, f32; f32 contexts may name
+ * `out` itself) and stats [batch, kv_heads, heads / kv_heads * queries, 2] are written.
+ * The backward pass takes the forward call's arguments (out may be NULL), dout (strides like q's) and writes dq and dk,
+ * dv, dense (dq, or dk and dv together, may be NULL); rows of dk / dv outside the masks are zeros.  kv heads shared by
+ * several query heads receive their sum.  The workspace call for it is made with dq, dk and dv set. */
 typedef struct tapir_attn_args {
   int64_t batch, queries, keys;
   int heads, kv_heads, dim;
@@ -452,7 +453,7 @@ typedef struct tapir_attn_args {
   const int32_t* key_lengths;
   const uint8_t* key_mask;
   void* out;
-  float *out_f32, *lse;
+  float *out_f32, *stats;
   const void* dout;
   int64_t dout_stride[3];
   void *dq, *dk, *dv;

@@ -70,7 +70,7 @@ class TapirAttnArgs(ctypes.Structure):   # tapir_attn_args
               ('q', c_void_p), ('k', c_void_p), ('v', c_void_p),
               ('q_stride', c_int64 * 3), ('k_stride', c_int64 * 3), ('v_stride', c_int64 * 3),
               ('key_lengths', c_void_p), ('key_mask', c_void_p), ('out', c_void_p), ('out_f32', c_void_p),
-              ('lse', c_void_p), ('dout', c_void_p), ('dout_stride', c_int64 * 3),
+              ('stats', c_void_p), ('dout', c_void_p), ('dout_stride', c_int64 * 3),
               ('dq', c_void_p), ('dk', c_void_p), ('dv', c_void_p), ('workspace', c_void_p),
               ('workspace_bytes', c_uint64)]
 

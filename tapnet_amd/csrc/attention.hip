@@ -86,33 +86,51 @@ void ln_bwd_dispatch(const LnBwdArgs& a, unsigned grid, hipStream_t s) {
 
 // ---------------------------------------------------------------------------------------------------- attention
 int attn_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int attn_row_step(int dtype, int dp) { return 32L * dp * (dtype == TAPIR_BF16 ? 2 : 4) / 16 >= AT_THREADS ? 32 : 64; }   // AtRowTile
 
 struct AttnPlan {
-  int dp, row_tiles, splits, tiles_per_split;
-  size_t part_o, part_ml;   // floats
+  int dp, row_tiles, splits, tiles_per_split, row_splits, row_steps_per_split;
+  size_t part_o, part_ml, delta, part_dq, part_dkv;   // floats
 };
 
-// Key splits of the forward pass: where the row tiles alone leave compute units idle, the keys are cut until there are about
-// four workgroups a CU, each with four tiles at least (the join reads splits x rows partial results).
-AttnPlan attn_plan(const tapir_attn_args* a, int dtype) {
-  AttnPlan p{};
-  const int kt = dtype == TAPIR_BF16 ? 64 : 32;
-  p.dp = attn_pad(a->dim);
-  const long rows = (long)(a->heads / a->kv_heads) * a->queries;
-  p.row_tiles = (int)((rows + AT_QROWS - 1) / AT_QROWS);
-  const long tiles = std::max<long>(1, (a->keys + kt - 1) / kt);
-  const long base = std::max<long>(1, (long)a->batch * a->kv_heads * p.row_tiles);
-  long s = std::min<long>((1024 + base - 1) / base, (tiles + 3) / 4);
+size_t round4(size_t n) { return (n + 3) & ~(size_t)3; }   // (shares of a workspace start at multiples of 16 bytes)
+
+// Splits of a long axis: where the tiles of the other one alone leave compute units idle (`base` workgroups), it is cut until
+// there are `want`, each of `least` steps at least (the join reads a partial result per split).
+void attn_split(long steps, long base, long want, long least, int* splits, int* per) {
+  long s = std::min<long>((want + base - 1) / base, (steps + least - 1) / least);
   s = std::max<long>(1, std::min<long>(s, 1024));
-  p.tiles_per_split = (int)((tiles + s - 1) / s);
-  p.splits = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
-  if (p.splits > 1) {
-    const size_t r = (size_t)p.splits * a->batch * a->kv_heads * rows;
-    p.part_o = r * p.dp;
-    p.part_ml = r * 2;
+  *per = (int)((steps + s - 1) / s);
+  *splits = (int)((steps + *per - 1) / *per);
+}
+
+AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
+  AttnPlan p{};
+  const bool bf16 = dtype == TAPIR_BF16;
+  p.dp = attn_pad(a->dim);
+  const long rows = (long)(a->heads / a->kv_heads) * a->queries, heads = std::max<long>(1, (long)a->batch * a->kv_heads);
+  p.row_tiles = (int)((rows + AT_QROWS - 1) / AT_QROWS);
+  const int kt = bf16 ? 64 : 32;
+  const long tiles = std::max<long>(1, (a->keys + kt - 1) / kt);
+  attn_split(tiles, std::max<long>(1, heads * p.row_tiles), backward ? 512 : 1024, 4, &p.splits, &p.tiles_per_split);
+  if (!backward) {
+    if (p.splits > 1) {
+      const size_t r = (size_t)p.splits * a->batch * a->kv_heads * rows;
+      p.part_o = r * p.dp;
+      p.part_ml = round4(r * 2);
+    }
+    return p;
   }
+  const int rt = attn_row_step(dtype, p.dp);
+  attn_split(std::max<long>(1, (rows + rt - 1) / rt), std::max<long>(1, heads * ((a->keys + AT_KEYS - 1) / AT_KEYS)), 512, 4,
+             &p.row_splits, &p.row_steps_per_split);
+  p.delta = round4((size_t)heads * rows);
+  if (p.splits > 1 && a->dq) p.part_dq = (size_t)p.splits * a->batch * a->queries * a->heads * a->dim;
+  if (p.row_splits > 1 && a->dk) p.part_dkv = (size_t)p.row_splits * a->batch * a->keys * a->kv_heads * a->dim;
   return p;
 }
+
+size_t attn_workspace_floats(const AttnPlan& p) { return p.part_o + p.part_ml + p.delta + p.part_dq + 2 * p.part_dkv; }
 
 int attn_check(tapir_ctx* c, const tapir_attn_args* a, bool backward) {
   OP_REQUIRE(c, a != nullptr, TAPIR_ERR_INVALID, "cross_attention: null arguments");
@@ -138,13 +156,13 @@ int attn_check(tapir_ctx* c, const tapir_attn_args* a, bool backward) {
              TAPIR_ERR_INVALID, "cross_attention: null tensor, or one whose rows do not start at multiples of 16 bytes");
   OP_REQUIRE(c, no_q || (a->out && aligned16(a->out)) || backward, TAPIR_ERR_INVALID, "cross_attention: null or misaligned output");
   if (backward) {
-    OP_REQUIRE(c, no_q || (a->dq && aligned16(a->dq) && a->out_f32 && aligned16(a->out_f32) && a->lse), TAPIR_ERR_INVALID,
-               "cross_attention: the backward pass needs out_f32 and lse of the forward pass, and dq");
-    OP_REQUIRE(c, no_k || (a->dk && a->dv && aligned16(a->dk) && aligned16(a->dv)), TAPIR_ERR_INVALID,
-               "cross_attention: the backward pass needs dk and dv");
+    OP_REQUIRE(c, no_q || (a->out_f32 && aligned16(a->out_f32) && a->stats && aligned16(a->stats)), TAPIR_ERR_INVALID,
+               "cross_attention: the backward pass needs out_f32 and stats of the forward pass");
+    OP_REQUIRE(c, aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv) && (a->dk == nullptr) == (a->dv == nullptr), TAPIR_ERR_INVALID,
+               "cross_attention: misaligned gradients, or one of dk and dv without the other");
   } else {
-    OP_REQUIRE(c, (a->out_f32 == nullptr) == (a->lse == nullptr) && aligned16(a->out_f32), TAPIR_ERR_INVALID,
-               "cross_attention: out_f32 and lse go together");
+    OP_REQUIRE(c, (a->out_f32 == nullptr) == (a->stats == nullptr) && aligned16(a->out_f32) && aligned16(a->stats), TAPIR_ERR_INVALID,
+               "cross_attention: out_f32 and stats go together");
   }
   return TAPIR_OK;
 }
@@ -154,11 +172,19 @@ AttnArgs attn_args(const tapir_attn_args* a, const AttnPlan& p) {
   k.q = a->q; k.k = a->k; k.v = a->v; k.dout = a->dout;
   for (int i = 0; i < 3; ++i) { k.qs[i] = a->q_stride[i]; k.ks[i] = a->k_stride[i]; k.vs[i] = a->v_stride[i]; k.ds[i] = a->dout_stride[i]; }
   k.key_lengths = a->key_lengths; k.key_mask = a->key_mask;
-  k.out = a->out; k.out32 = a->out_f32; k.lse = a->lse; k.dq = a->dq; k.dk = a->dk; k.dv = a->dv;
+  k.out = a->out; k.out32 = a->out_f32; k.stats = a->stats; k.dq = a->dq; k.dk = a->dk; k.dv = a->dv;
   k.B = a->batch; k.Hkv = a->kv_heads; k.G = a->heads / a->kv_heads; k.D = a->dim;
   k.Nq = a->queries; k.Nk = a->keys; k.rows = (long)k.G * a->queries;
   k.scale = a->scale; k.scale2 = a->scale * kLog2e;
   k.splits = p.splits; k.tiles_per_split = p.tiles_per_split; k.row_tiles = p.row_tiles;
+  k.row_splits = p.row_splits; k.row_steps_per_split = p.row_steps_per_split;
+  k.n_dq = (long)a->batch * a->queries * a->heads * a->dim;
+  k.n_dkv = (long)a->batch * a->keys * a->kv_heads * a->dim;
+  float* w = (float*)a->workspace;
+  if (p.part_o) { k.part_o = w; k.part_ml = w + p.part_o; w += p.part_o + p.part_ml; }
+  k.delta = w; w += p.delta;
+  if (p.part_dq) { k.part_dq = w; w += p.part_dq; }
+  if (p.part_dkv) { k.part_dk = w; k.part_dv = w + p.part_dkv; }
   return k;
 }
 
@@ -174,14 +200,19 @@ void attn_fwd_launch(const AttnArgs& k, hipStream_t s) {
 
 template <typename T, int DP>
 void attn_bwd_launch(const AttnArgs& k, hipStream_t s) {
-  if (k.rows > 0) {
-    const unsigned grid = (unsigned)((long)k.B * k.Hkv * k.row_tiles);
+  if (k.rows > 0 && k.dq) {
+    const unsigned grid = (unsigned)((long)k.B * k.Hkv * k.row_tiles * k.splits);
     hipLaunchKernelGGL((attn_dq_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
+  } else if (k.rows > 0) {
+    const long rows = (long)k.B * k.Hkv * k.rows;
+    hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k);
   }
-  if (k.Nk > 0) {
-    const unsigned grid = (unsigned)((long)k.B * k.Hkv * ((k.Nk + AT_KEYS - 1) / AT_KEYS));
+  if (k.Nk > 0 && k.dk) {
+    const unsigned grid = (unsigned)((long)k.B * k.Hkv * ((k.Nk + AT_KEYS - 1) / AT_KEYS) * k.row_splits);
     hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
   }
+  const long join = (k.part_dq ? k.n_dq : 0) + (k.part_dk ? 2 * k.n_dkv : 0);
+  if (join > 0) hipLaunchKernelGGL((attn_join_grads_kernel<T>), dim3(stride_grid((join / 4 + AT_THREADS - 1) / AT_THREADS)), dim3(AT_THREADS), 0, s, k);
 }
 
 #define ATTN_DISPATCH(fn, dtype, dp, ...)                                                                              \
@@ -192,8 +223,6 @@ void attn_bwd_launch(const AttnArgs& k, hipStream_t s) {
       if ((dp) == 32) fn<float, 32>(__VA_ARGS__); else if ((dp) == 64) fn<float, 64>(__VA_ARGS__); else fn<float, 128>(__VA_ARGS__);    \
     }                                                                                                                  \
   } while (0)
-
-size_t attn_backward_floats(const tapir_attn_args* a) { return (size_t)a->batch * a->heads * a->queries; }
 
 }  // namespace
 
@@ -232,7 +261,7 @@ int tapir_layer_norm_backward(tapir_ctx* c, const void* x, int64_t x_stride, con
   if (!c) return TAPIR_ERR_INVALID;
   const CtxInfo ci = ctx_info(c);
   OP_REQUIRE(c, rows >= 0 && channels >= 1, TAPIR_ERR_INVALID, "layer_norm: bad size");
-  OP_REQUIRE(c, rows == 0 || (x && dy && mean && rstd && dx), TAPIR_ERR_INVALID, "layer_norm: null tensor");
+  OP_REQUIRE(c, rows == 0 || (x && dy && mean && rstd), TAPIR_ERR_INVALID, "layer_norm: null tensor");
   const int ept = ln_ept(ci.dtype, channels, x_stride, x, dy_stride, dy, dx);
   const unsigned grid = ln_bwd_grid(rows, channels, ept);
   const bool params = dgamma || dbeta;
@@ -298,8 +327,7 @@ int tapir_cross_attention_workspace(tapir_ctx* c, const tapir_attn_args* a, int 
   if (!c) return TAPIR_ERR_INVALID;
   OP_REQUIRE(c, a && bytes && a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->kv_heads >= 1 && a->heads >= 1 &&
                     a->heads % a->kv_heads == 0, TAPIR_ERR_INVALID, "cross_attention: bad size");
-  const AttnPlan p = attn_plan(a, ctx_info(c).dtype);
-  *bytes = sizeof(float) * (backward ? attn_backward_floats(a) : p.part_o + p.part_ml);
+  *bytes = sizeof(float) * attn_workspace_floats(attn_plan(a, ctx_info(c).dtype, backward != 0));
   return TAPIR_OK;
 }
 
@@ -309,13 +337,12 @@ int tapir_cross_attention(tapir_ctx* c, const tapir_attn_args* a, void* stream) 
   const int rc = attn_check(c, a, false);
   if (rc != TAPIR_OK) return rc;
   if (a->batch == 0 || a->queries == 0) return TAPIR_OK;
-  const AttnPlan p = attn_plan(a, ci.dtype);
-  OP_REQUIRE(c, p.splits == 1 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= sizeof(float) * (p.part_o + p.part_ml)),
+  const AttnPlan p = attn_plan(a, ci.dtype, false);
+  const size_t floats = attn_workspace_floats(p);
+  OP_REQUIRE(c, floats == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= sizeof(float) * floats),
              TAPIR_ERR_INVALID, "cross_attention: workspace missing or too small (tapir_cross_attention_workspace)");
   OP_TRY(c, hipSetDevice(ci.device));
-  AttnArgs k = attn_args(a, p);
-  k.part_o = (float*)a->workspace;
-  k.part_ml = (float*)a->workspace + p.part_o;
+  const AttnArgs k = attn_args(a, p);
   ATTN_DISPATCH(attn_fwd_launch, ci.dtype, p.dp, k, (hipStream_t)stream);
   OP_TRY(c, hipGetLastError());
   return TAPIR_OK;
@@ -327,12 +354,12 @@ int tapir_cross_attention_backward(tapir_ctx* c, const tapir_attn_args* a, void*
   const int rc = attn_check(c, a, true);
   if (rc != TAPIR_OK) return rc;
   if (a->batch == 0) return TAPIR_OK;
-  OP_REQUIRE(c, a->queries == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= sizeof(float) * attn_backward_floats(a)),
+  const AttnPlan p = attn_plan(a, ci.dtype, true);
+  const size_t floats = attn_workspace_floats(p);
+  OP_REQUIRE(c, floats == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= sizeof(float) * floats),
              TAPIR_ERR_INVALID, "cross_attention: workspace missing or too small (tapir_cross_attention_workspace)");
   OP_TRY(c, hipSetDevice(ci.device));
-  const AttnPlan p = attn_plan(a, ci.dtype);
-  AttnArgs k = attn_args(a, p);
-  k.delta = (float*)a->workspace;
+  const AttnArgs k = attn_args(a, p);
   ATTN_DISPATCH(attn_bwd_launch, ci.dtype, p.dp, k, (hipStream_t)stream);
   OP_TRY(c, hipGetLastError());
   return TAPIR_OK;

@@ -1,6 +1,6 @@
 // Cross attention of query rows to an encoder's tokens, forward and backward, one pass over the keys.
 //
-//   s_rk = scale q_r . k_k,  p_rk = exp(s_rk - L_r),  L_r = log sum_k exp(s_rk),  o_r = sum_k p_rk v_k
+//   s_rk = scale q_r . k_k,  p_rk = exp(s_rk - m_r) / l_r,  l_r = sum_k exp(s_rk - m_r),  o_r = sum_k p_rk v_k
 //   D_r = do_r . o_r,  dp_rk = do_r . v_k,  ds_rk = p_rk (dp_rk - D_r) scale
 //   dq_r = sum_k ds_rk k_k,   dk_k = sum_r ds_rk q_r,   dv_k = sum_r p_rk do_r
 //
@@ -29,6 +29,7 @@ constexpr int AT_THREADS = 64 * AT_WAVES;
 constexpr int AT_QROWS = 32 * AT_WAVES;      // query rows of a forward / dq workgroup
 constexpr int AT_KEYS = 32 * AT_WAVES;       // keys of a dk / dv workgroup
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float AT_SLACK = 8.f;
 
 struct AttnArgs {
   const void *q, *k, *v, *dout;
@@ -37,13 +38,16 @@ struct AttnArgs {
   const unsigned char* key_mask;       // [B, Nk] or null: nonzero = may be attended to
   void* out;                           // [B, Nq, H, D] dense
   float *out32;                        // the same unrounded (training), or null
-  float *lse;                          // [B, Hkv, G * Nq]: L_r in powers of two (0 for a row without keys), or null
-  float *delta;                        // [B, Hkv, G * Nq]: D_r
+  float *stats;                        // [B, Hkv, rows, 2]: m_r log2(e) and 1 / l_r (0, 0 for a row without keys), or null
+  float *delta;                        // [B, Hkv, rows]: D_r
   void *dq, *dk, *dv;                  // dense
-  float *part_o, *part_ml;             // split keys: [splits, B * Hkv, rows, DP] and [splits, B * Hkv, rows, 2]
+  float *part_o, *part_ml;             // split keys, forward: [splits, B * Hkv, rows, DP] and [splits, B * Hkv, rows, 2]
+  float *part_dq, *part_dk, *part_dv;  // backward: [splits] copies of dq (keys split) and of dk, dv (rows split) in f32
+  long n_dq, n_dkv;                    // elements of dq and of dk
   long Nq, Nk, rows;                   // rows = G * Nq
   int B, Hkv, G, D;
-  int splits, tiles_per_split;         // key tiles of a split
+  int splits, tiles_per_split;         // key tiles of a split (forward, dq)
+  int row_splits, row_steps_per_split; // row steps of a split (dk / dv)
   int row_tiles;
   float scale, scale2;                 // scale, scale * log2(e)
 };
@@ -121,7 +125,7 @@ __device__ __forceinline__ void at_mma_tr(f32x16& c, const float* X, int r0, int
 }
 
 // the 16 values of a lane as the operand of at_mma_tr: rounded to bf16 (the products of the next sum take bf16 operands; the
-// relative error 2^-9 of each term is the size of the output's own rounding and averages out over the sum), or as they are
+// relative error of each term, 2^-8 at most, is the size of the output's own rounding and averages out over the sum), or as they are
 __device__ __forceinline__ void at_operand(const f32x16& p, unsigned (&w)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
   f32x16 o[NB];
 #pragma unroll
   for (int d = 0; d < NB; ++d) o[d] = at_zero();
-  float m = -INFINITY, sum = 0.f;
+  float base = -INFINITY, sum = 0.f;   // base: of the exponentials, in powers of two
 
   uint64_t bits = 0;
   auto stage = [&](int t, int buf) {
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
     __syncthreads();
     if (t + 1 < t1) stage(t + 1, buf ^ 1);
     f32x16 s[KT / 32];
-    float top = m;
+    float top = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       s[kb] = at_zero();
@@ -264,20 +268,25 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
     }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float base = top == -INFINITY ? 0.f : top * a.scale2;
-    const float alpha = fast_exp2(fmaf(m, a.scale2, -base));
-    m = top;
-    sum *= alpha;
+    // The base of the exponentials need not be the running maximum itself: it stays until a score is AT_SLACK powers of two above
+    // it (sums and products stay below 2^AT_SLACK per key, far from f32's range), which spares nearly all rescaling of o.
+    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2;
+    const bool move = top > base + AT_SLACK;          // (base -inf: every finite score moves it)
+    if (__ballot(move) != 0) {
+      const float alpha = move ? fast_exp2(base - top) : 1.f;
+      if (move) base = top;
+      sum *= alpha;
 #pragma unroll
-    for (int d = 0; d < NB; ++d)
+      for (int d = 0; d < NB; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+    }
+    const float off = base == -INFINITY ? 0.f : base;
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -base));
+        s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -off));
         sum += s[kb][i];
       }
       AtOperand<T> p;
@@ -297,7 +306,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         at_store4<float>(po + d * 32 + 8 * i + 4 * h, o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
-    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m == -INFINITY ? m : m * a.scale2, sum);
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(base, sum);
     return;
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
@@ -310,10 +319,10 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
       if (c < a.D) {
         const float x = o[d][4 * i] * inv, y = o[d][4 * i + 1] * inv, z = o[d][4 * i + 2] * inv, u = o[d][4 * i + 3] * inv;
         at_store4<T>((T*)a.out + at + c, x, y, z, u);
-        if (a.out32) at_store4<float>(a.out32 + at + c, x, y, z, u);
+        if (a.out32 && (const void*)a.out32 != a.out) at_store4<float>(a.out32 + at + c, x, y, z, u);
       }
     }
-  if (a.lse && h == 0) a.lse[bh * a.rows + row] = sum > 0.f ? fmaf(m, a.scale2, log2f(sum)) : 0.f;
+  if (a.stats && h == 0) *reinterpret_cast<float2*>(a.stats + 2 * (bh * a.rows + row)) = make_float2(base == -INFINITY ? 0.f : base, inv);
 }
 
 // joins the key splits: a wave a row;  o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s
@@ -342,13 +351,14 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a, int D
       x = fmaf(fast_exp2(a.part_ml[2 * (s * total + r)] - base), a.part_o[(s * total + r) * DP + c], x);
     x *= inv;
     Elem<T>::st((T*)a.out + at + c, x);
-    if (a.out32) a.out32[at + c] = x;
+    if (a.out32 && (const void*)a.out32 != a.out) a.out32[at + c] = x;
   }
-  if (a.lse && l == 0) a.lse[r] = sum > 0.f ? base + log2f(sum) : 0.f;
+  if (a.stats && l == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(base, inv);
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward
-// dq (and D_r on the way): the forward kernel's loop with p from the saved L_r.
+// dq (and D_r on the way): the forward kernel's loop with p from the saved statistics; 1 / l_r is a factor of the whole row and
+// joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
@@ -357,6 +367,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
   long w = at_work_index();
   const int rt = (int)(w % a.row_tiles); w /= a.row_tiles;
+  const int split = (int)(w % a.splits); w /= a.splits;
   const int hk = (int)(w % a.Hkv), b = (int)(w / a.Hkv);
   const long row = (long)rt * AT_QROWS + wave * 32 + (l & 31);
   const bool live = row < a.rows;
@@ -364,7 +375,9 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
   const int head = hk * a.G + (int)(rr / a.Nq);
   const long query = rr % a.Nq;
   const long len = at_key_len(a, b);
-  const int n_tiles = (int)((len + KT - 1) / KT);
+  const int t0 = split * a.tiles_per_split;
+  const long n_tiles = (len + KT - 1) / KT;
+  const int t1 = (int)(n_tiles < (long)t0 + a.tiles_per_split ? n_tiles : (long)t0 + a.tiles_per_split);
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
   const long bh = (long)b * a.Hkv + hk;
@@ -386,8 +399,8 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
     }
   }
   delta += __shfl_xor(delta, 32);
-  const float lse = a.lse[bh * a.rows + rr];
-  if (live && h == 0) a.delta[bh * a.rows + row] = delta;
+  const float2 stat = *reinterpret_cast<const float2*>(a.stats + 2 * (bh * a.rows + rr));
+  if (live && h == 0 && split == 0) a.delta[bh * a.rows + row] = delta;
   f32x16 o[NB];
 #pragma unroll
   for (int d = 0; d < NB; ++d) o[d] = at_zero();
@@ -399,13 +412,13 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
     at_stage<T, KT, DP>(kt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? kp + (k0 + r) * a.ks[1] : (const T*)nullptr; });
     at_stage<T, KT, DP>(vt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? vp + (k0 + r) * a.vs[1] : (const T*)nullptr; });
   };
-  if (n_tiles > 0) stage(0, 0);
-  for (int t = 0; t < n_tiles; ++t) {
-    const int buf = t & 1;
+  if (t0 < t1) stage(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
     const uint64_t cur = bits;
     dma_wait<0>();
     __syncthreads();
-    if (t + 1 < n_tiles) stage(t + 1, buf ^ 1);
+    if (t + 1 < t1) stage(t + 1, buf ^ 1);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       f32x16 s = at_zero(), g = at_zero();
@@ -417,7 +430,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
       const unsigned mine = (unsigned)(cur >> (32 * kb)) >> (4 * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float p = fast_exp2(fmaf(s[i], a.scale2, -lse)) * (g[i] - delta);
+        const float p = fast_exp2(fmaf(s[i], a.scale2, -stat.x)) * (g[i] - delta);
         s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? p : 0.f;
       }
       AtOperand<T> p;
@@ -427,28 +440,47 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
     }
   }
   if (!live) return;
+  const float f = stat.y * a.scale;
 #pragma unroll
   for (int d = 0; d < NB; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int c = d * 32 + 8 * i + 4 * h;
-      if (c < a.D)
-        at_store4<T>((T*)a.dq + at + c, o[d][4 * i] * a.scale, o[d][4 * i + 1] * a.scale, o[d][4 * i + 2] * a.scale,
-                     o[d][4 * i + 3] * a.scale);
+      if (c < a.D) {
+        const float x = o[d][4 * i] * f, y = o[d][4 * i + 1] * f, z = o[d][4 * i + 2] * f, u = o[d][4 * i + 3] * f;
+        if (a.splits > 1) at_store4<float>(a.part_dq + split * a.n_dq + at + c, x, y, z, u);
+        else at_store4<T>((T*)a.dq + at + c, x, y, z, u);
+      }
     }
 }
 
-// dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads, RT at a time.
+// D_r where dq is not wanted: a wave a row
+template <typename T>
+__global__ __launch_bounds__(AT_THREADS) void attn_delta_kernel(AttnArgs a) {
+  const long total = (long)a.B * a.Hkv * a.rows, r = (long)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
+  if (r >= total) return;
+  const int l = threadIdx.x & 63;
+  const long bh = r / a.rows, row = r % a.rows, b = bh / a.Hkv, head = bh % a.Hkv * a.G + row / a.Nq, query = row % a.Nq;
+  const T* gp = (const T*)a.dout + b * a.ds[0] + query * a.ds[1] + head * a.ds[2];
+  const float* op = a.out32 + ((b * a.Nq + query) * a.Hkv * a.G + head) * a.D;
+  float delta = 0.f;
+  for (int c = l; c < a.D; c += 64) delta = fmaf(Elem<T>::ld(gp + c), op[c], delta);
+  delta = wave_sum(delta);
+  if (l == 0) a.delta[r] = delta;
+}
+
+// dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads (or a split of them), RT at a time.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
   __shared__ __attribute__((aligned(16))) T qt[2][RT * DP];
   __shared__ __attribute__((aligned(16))) T gt[2][RT * DP];
-  __shared__ __attribute__((aligned(16))) float ld[2][2][RT];   // L_r, D_r
+  __shared__ __attribute__((aligned(16))) float ld[2][3][RT];   // m_r, 1 / l_r, D_r
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
   const long key_tiles = (a.Nk + AT_KEYS - 1) / AT_KEYS;
   long w = at_work_index();
   const long kt = w % key_tiles; w /= key_tiles;
+  const int split = (int)(w % a.row_splits); w /= a.row_splits;
   const int hk = (int)(w % a.Hkv), b = (int)(w / a.Hkv);
   const long key = kt * AT_KEYS + wave * 32 + (l & 31);
   const long len = at_key_len(a, b);
@@ -468,7 +500,8 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
   for (int d = 0; d < NB; ++d) { dk[d] = at_zero(); dv[d] = at_zero(); }
   // (a tile behind the clip's length has nothing to add: no steps, zeros are stored)
-  const int n_tiles = kt * AT_KEYS < len ? (int)((a.rows + RT - 1) / RT) : 0;
+  const int t0 = split * a.row_steps_per_split, n_steps = kt * AT_KEYS < len ? (int)((a.rows + RT - 1) / RT) : 0;
+  const int t1 = n_steps < t0 + a.row_steps_per_split ? n_steps : t0 + a.row_steps_per_split;
   auto stage = [&](int t, int buf) {
     const long r0 = (long)t * RT;
     at_stage<T, RT, DP>(qt[buf], a.D, [&](int r) {
@@ -479,18 +512,23 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
       const long row = r0 + r;
       return row < a.rows ? (const T*)a.dout + b * a.ds[0] + (row % a.Nq) * a.ds[1] + (hk * a.G + row / a.Nq) * a.ds[2] : (const T*)nullptr;
     });
-    if (threadIdx.x < 2 * RT) {
-      const long row = r0 + (threadIdx.x & (RT - 1));
-      const float* src = threadIdx.x < RT ? a.lse : a.delta;
-      ld[buf][threadIdx.x / RT][threadIdx.x & (RT - 1)] = row < a.rows ? src[bh * a.rows + row] : 0.f;
+    if (threadIdx.x < RT) {
+      const long row = r0 + threadIdx.x;
+      float2 st = make_float2(0.f, 0.f);
+      if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + 2 * (bh * a.rows + row));
+      ld[buf][0][threadIdx.x] = st.x;
+      ld[buf][1][threadIdx.x] = st.y;
+    } else if (threadIdx.x < 2 * RT) {
+      const long row = r0 + (threadIdx.x - RT);
+      ld[buf][2][threadIdx.x - RT] = row < a.rows ? a.delta[bh * a.rows + row] : 0.f;
     }
   };
-  if (n_tiles > 0) stage(0, 0);
-  for (int t = 0; t < n_tiles; ++t) {
-    const int buf = t & 1;
+  if (t0 < t1) stage(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
     dma_wait<0>();
     __syncthreads();
-    if (t + 1 < n_tiles) stage(t + 1, buf ^ 1);
+    if (t + 1 < t1) stage(t + 1, buf ^ 1);
 #pragma unroll
     for (int rb = 0; rb < RT; rb += 32) {
       f32x16 s = at_zero(), g = at_zero();
@@ -501,12 +539,13 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 L = *reinterpret_cast<const float4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
-        const float4 E = *reinterpret_cast<const float4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
-        const float Lv[4] = {L.x, L.y, L.z, L.w}, Ev[4] = {E.x, E.y, E.z, E.w};
+        const float4 M = *reinterpret_cast<const float4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
+        const float4 I = *reinterpret_cast<const float4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
+        const float4 E = *reinterpret_cast<const float4*>(&ld[buf][2][rb + 8 * i + 4 * h]);
+        const float Mv[4] = {M.x, M.y, M.z, M.w}, Iv[4] = {I.x, I.y, I.z, I.w}, Ev[4] = {E.x, E.y, E.z, E.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = in ? fast_exp2(fmaf(s[4 * i + j], a.scale2, -Lv[j])) : 0.f;
+          const float p = in ? fast_exp2(fmaf(s[4 * i + j], a.scale2, -Mv[j])) * Iv[j] : 0.f;
           s[4 * i + j] = p;
           g[4 * i + j] = p * (g[4 * i + j] - Ev[j]);
         }
@@ -529,11 +568,38 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
     for (int i = 0; i < 4; ++i) {
       const int c = d * 32 + 8 * i + 4 * h;
       if (c < a.D) {
-        at_store4<T>((T*)a.dk + at + c, dk[d][4 * i] * a.scale, dk[d][4 * i + 1] * a.scale, dk[d][4 * i + 2] * a.scale,
-                     dk[d][4 * i + 3] * a.scale);
-        at_store4<T>((T*)a.dv + at + c, dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]);
+        float x[4], y[4];   // (a masked key: zeros, also where dout holds something that is not finite)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[j] = in ? dk[d][4 * i + j] * a.scale : 0.f; y[j] = in ? dv[d][4 * i + j] : 0.f; }
+        if (a.row_splits > 1) {
+          at_store4<float>(a.part_dk + split * a.n_dkv + at + c, x[0], x[1], x[2], x[3]);
+          at_store4<float>(a.part_dv + split * a.n_dkv + at + c, y[0], y[1], y[2], y[3]);
+        } else {
+          at_store4<T>((T*)a.dk + at + c, x[0], x[1], x[2], x[3]);
+          at_store4<T>((T*)a.dv + at + c, y[0], y[1], y[2], y[3]);
+        }
       }
     }
+}
+
+// adds the splits' shares of a gradient, in order (4 elements a thread; every row has a multiple of 8)
+template <typename T>
+__device__ __forceinline__ void at_add_shares(T* out, const float* part, long n, int shares, long i) {
+  float4 s = *reinterpret_cast<const float4*>(part + i);
+  for (int p = 1; p < shares; ++p) {
+    const float4 v = *reinterpret_cast<const float4*>(part + p * n + i);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  at_store4<T>(out + i, s.x, s.y, s.z, s.w);
+}
+template <typename T>
+__global__ __launch_bounds__(AT_THREADS) void attn_join_grads_kernel(AttnArgs a) {
+  const long nq = a.part_dq ? a.n_dq : 0, nk = a.part_dk ? a.n_dkv : 0;
+  for (long i = 4 * ((long)blockIdx.x * AT_THREADS + threadIdx.x); i < nq + 2 * nk; i += 4L * gridDim.x * AT_THREADS) {
+    if (i < nq) at_add_shares((T*)a.dq, a.part_dq, a.n_dq, a.splits, i);
+    else if (i < nq + nk) at_add_shares((T*)a.dk, a.part_dk, a.n_dkv, a.row_splits, i - nq);
+    else at_add_shares((T*)a.dv, a.part_dv, a.n_dkv, a.row_splits, i - nq - nk);
+  }
 }
 
 }  // namespace tapir

@@ -44,3 +44,12 @@ done
 for p in $PIDS; do wait $p; done
 hipcc --offload-arch=gfx950 -fPIC -shared build/engine.o build/attention.o -o libtapir_hip.so
 python3 check_packed_forms.py libtapir_hip.so
+# the operators on torch tensors (host code: argument checks, autograd nodes)
+TORCH=$(python3 -c "import importlib.util, os; print(os.path.dirname(importlib.util.find_spec('torch').origin))")
+PYINC=$(python3 -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+if [ "$UNITS" == "engine attention" ] || [ torch_ops.cpp -nt ../_torch_ops.so ] || [ ../../include/tapir_hip.h -nt ../_torch_ops.so ]; then
+  g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -DTORCH_EXTENSION_NAME=_torch_ops \
+    -isystem "$TORCH/include" -isystem "$TORCH/include/torch/csrc/api/include" -isystem /opt/rocm/include -isystem "$PYINC" \
+    torch_ops.cpp -o ../_torch_ops.so -L. -ltapir_hip -L"$TORCH/lib" -ltorch -ltorch_cpu -ltorch_hip -ltorch_python -lc10 -lc10_hip \
+    -Wl,-rpath,'$ORIGIN/csrc'
+fi

@@ -28,7 +28,7 @@ struct LnBwdArgs {
   const void* dy; long lddy;
   const float* gamma;
   const float *mean, *rstd;
-  void* dx;                       // [rows, C] dense
+  void* dx;                       // [rows, C] dense, or null
   float* part;                    // [grid][2][C] partial sums of dgamma, dbeta (null: neither is wanted)
   long rows; int C;
 };
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_kernel(LnBwdArgs a)
     }
     sg = ln_sum<LPR>(sg) * inv;
     su = ln_sum<LPR>(su) * inv;
-    if (!live) continue;
+    if (!live || !a.dx) continue;
     T* op = (T*)a.dx + row * a.C;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -266,6 +266,7 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_long_kernel(LnBwdAr
     }
     sg = ln_block_sum(sg, red) * inv;
     su = ln_block_sum(su, red) * inv;
+    if (!a.dx) continue;
     T* op = (T*)a.dx + row * a.C;
     for (int c = threadIdx.x; c < a.C; c += LN_THREADS) {
       const float dy = Elem<T>::ld(yp + c), u = (Elem<T>::ld(xp + c) - mean) * rstd, g = a.gamma ? dy * a.gamma[c] : dy;

@@ -162,8 +162,8 @@ def run_attention(c, q, k, v, lengths=None, mask=None, scale=None, dout=None):
   out = aligned_empty(q.shape, q.dtype)
   a.out = out.data_ptr()
   if dout is not None:
-    out32, lse = aligned_empty(q.shape, torch.float32), aligned_empty(q.shape[:3], torch.float32)
-    a.out_f32, a.lse = out32.data_ptr(), lse.data_ptr()
+    out32, stats = aligned_empty(q.shape, torch.float32), aligned_empty((*q.shape[:3], 2), torch.float32)
+    a.out_f32, a.stats = out32.data_ptr(), stats.data_ptr()
   nbytes = ctypes.c_uint64()
   c('tapir_cross_attention_workspace', ctypes.byref(a), 0, ctypes.byref(nbytes))
   work = workspace(nbytes.value)
@@ -296,7 +296,7 @@ def test_refusals():
 
     def attend(backward=False, **changes):
       a = _ffi.TapirAttnArgs(1, 2, 2, 2, 1, 8, 1.0)
-      for n in ('q', 'k', 'v', 'out', 'out_f32', 'lse', 'dout', 'dq', 'dk', 'dv', 'workspace'):
+      for n in ('q', 'k', 'v', 'out', 'out_f32', 'stats', 'dout', 'dq', 'dk', 'dv', 'workspace'):
         setattr(a, n, p)
       a.workspace_bytes = 256
       for n in ('q', 'k', 'v', 'dout'):
@@ -315,9 +315,9 @@ def test_refusals():
                   dict(k_stride=9), dict(v_stride=7)):
         assert attend(back, **bad) == INV, bad
       assert attend(back, queries=1 << 31) == UNS and attend(back, keys=1 << 31) == UNS and attend(back, batch=1 << 22) == UNS
-    assert attend(out=None) == INV and attend(lse=None) == INV and attend(out_f32=None) == INV
-    assert attend(True, lse=None) == INV and attend(True, out_f32=None) == INV and attend(True, dk=None) == INV
-    assert attend(True, dq=None) == INV and attend(True, dout=None) == INV and attend(True, dout_stride=3) == INV
+    assert attend(out=None) == INV and attend(stats=None) == INV and attend(out_f32=None) == INV
+    assert attend(True, stats=None) == INV and attend(True, out_f32=None) == INV and attend(True, dk=None) == INV
+    assert attend(True, dv=None) == INV and attend(True, dout=None) == INV and attend(True, dout_stride=3) == INV
     assert attend(True, workspace=None) == INV and attend(True, workspace_bytes=4) == INV
     assert c.raw('tapir_cross_attention', None, None) == INV
     many = dict(keys=1 << 20, workspace=None)

@@ -392,7 +392,7 @@ def test_results_are_written_whole_and_nothing_else(A):
     setattr(a, name, t.data_ptr())
     getattr(a, name + '_stride')[:] = t.stride()[:3]
   frames = {n: framed(t.shape, t.dtype) for n, t in (('out', q), ('dq', q), ('dk', k), ('dv', v))}
-  frames['out_f32'], frames['lse'] = framed(q.shape, torch.float32), framed((2, 2, 66), torch.float32)
+  frames['out_f32'], frames['stats'] = framed(q.shape, torch.float32), framed((2, 2, 66, 2), torch.float32)
   for n, (_, t) in frames.items():
     setattr(a, n, t.data_ptr())
   stream = torch.cuda.current_stream().cuda_stream
