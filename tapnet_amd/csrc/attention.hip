@@ -194,7 +194,8 @@ void attn_fwd_launch(const AttnArgs& k, hipStream_t s) {
   hipLaunchKernelGGL((attn_fwd_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
   if (k.splits > 1) {
     const long rows = (long)k.B * k.Hkv * k.rows;
-    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k, DP);
+    if (k.splits >= 32) hipLaunchKernelGGL((attn_join_kernel<T, DP, AT_WAVES>), dim3((unsigned)rows), dim3(AT_THREADS), 0, s, k);
+    else hipLaunchKernelGGL((attn_join_kernel<T, DP, 1>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k);
   }
 }
 

@@ -41,7 +41,7 @@ struct AttnArgs {
   float *stats;                        // [B, Hkv, rows, 2]: m_r log2(e) and 1 / l_r (0, 0 for a row without keys), or null
   float *delta;                        // [B, Hkv, rows]: D_r
   void *dq, *dk, *dv;                  // dense
-  float *part_o, *part_ml;             // split keys, forward: [splits, B * Hkv, rows, DP] and [splits, B * Hkv, rows, 2]
+  float *part_o, *part_ml;             // split keys, forward: [splits, B * Hkv, rows, DP] and [B * Hkv, rows, splits, 2]
   float *part_dq, *part_dk, *part_dv;  // backward: [splits] copies of dq (keys split) and of dk, dv (rows split) in f32
   long n_dq, n_dkv;                    // elements of dq and of dk
   long Nq, Nk, rows;                   // rows = G * Nq
@@ -145,22 +145,29 @@ __device__ __forceinline__ f32x16 at_zero() {
   return z;
 }
 
-// ROWS x DP tile of a [token][channel] tensor -> LDS, 16-byte chunks, by the whole workgroup.  Row r of the tile is token
-// tok(r) (its address from `at`), or zeros where at() gives null; channels from D on are zeros too.
-template <typename T, int ROWS, int DP, class At>
-__device__ __forceinline__ void at_stage(T* lds, int D, const At& at) {
-  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, N = ROWS * CH / AT_THREADS;
+// ROWS x DP tile of a [token][channel] tensor -> LDS, 16-byte chunks, by the whole workgroup: thread i copies slots i, i + 256,
+// ... of the tile.  The offsets of a thread's chunks from the tile's first row stay the same for all tiles of a tensor.
+template <typename T, int ROWS, int DP> struct AtStage {
+  static constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, N = ROWS * CH / AT_THREADS;
   static_assert(ROWS * CH % AT_THREADS == 0, "tile");
-  const int wave = threadIdx.x >> 6;
+  long off[N];
+
+  static __device__ __forceinline__ int row(int n) { return (n * AT_THREADS + (int)threadIdx.x) / CH; }
+  static __device__ __forceinline__ int chunk(int n) { const int s = n * AT_THREADS + (int)threadIdx.x; return at_swizzle<CH>(s / CH, s % CH); }
+  __device__ __forceinline__ void init(long stride) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int slot = n * AT_THREADS + (int)threadIdx.x;
-    const int r = slot / CH, c = at_swizzle<CH>(r, slot % CH);
-    const T* p = at(r);
-    const void* src = p != nullptr && c * EPC < D ? (const void*)(p + c * EPC) : (const void*)at_zero16;
-    glds16(src, lds + (long)(n * AT_THREADS + wave * 64) * EPC);
+    for (int n = 0; n < N; ++n) off[n] = row(n) * stride + chunk(n) * EPC;
   }
-}
+  // a chunk from p, or zeros
+  static __device__ __forceinline__ void put(T* lds, int n, const T* p, bool ok) {
+    glds16(ok ? (const void*)p : (const void*)at_zero16, lds + (long)(n * AT_THREADS + (threadIdx.x >> 6) * 64) * EPC);
+  }
+  // rows from `first` on; row r is zeros where bit r of `bits` is not set, channels from D on are zeros too
+  __device__ __forceinline__ void rows(T* lds, const T* first, uint64_t bits, int D) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) put(lds, n, first + off[n], ((bits >> row(n)) & 1) && chunk(n) * EPC < D);
+  }
+};
 
 template <typename T, int CH> __device__ __forceinline__ uint4 at_chunk(const T* X, int r, int c) {
   return *reinterpret_cast<const uint4*>(X + ((long)r * CH + at_swizzle<CH>(r, c)) * AtFrag<T>::EPC);
@@ -201,11 +208,19 @@ template <typename T> struct AtTile { static constexpr int KT = sizeof(T) == 2 ?
 // query rows a dk / dv step stages: 32, or 64 where 32 rows are less than a copy per thread
 template <typename T, int DP> struct AtRowTile { static constexpr int RT = 32 * DP * (int)sizeof(T) / 16 >= AT_THREADS ? 32 : 64; };
 
+// waves per SIMD that the register allocation aims at
+template <typename T, int DP> struct AtWaves {
+  static constexpr bool BF16 = sizeof(T) == 2;
+  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? 3 : (BF16 ? 2 : 1);
+  static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : (BF16 ? 2 : 1);
+  static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
+};
+
 // ---------------------------------------------------------------------------------------------------------------- forward
 // A workgroup: AT_QROWS query rows of one key head, `tiles_per_split` key tiles; two LDS buffers, the next tile's copies in
 // flight under the current tile's products.
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
   __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
@@ -238,12 +253,15 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
   for (int d = 0; d < NB; ++d) o[d] = at_zero();
   float base = -INFINITY, sum = 0.f;   // base: of the exponentials, in powers of two
 
+  AtStage<T, KT, DP> sk, sv;
+  sk.init(a.ks[1]);
+  sv.init(a.vs[1]);
   uint64_t bits = 0;
   auto stage = [&](int t, int buf) {
     const long k0 = (long)t * KT;
     bits = at_key_bits(a, b, k0, len);
-    at_stage<T, KT, DP>(kt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? kp + (k0 + r) * a.ks[1] : (const T*)nullptr; });
-    at_stage<T, KT, DP>(vt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? vp + (k0 + r) * a.vs[1] : (const T*)nullptr; });
+    sk.rows(kt[buf], kp + k0 * a.ks[1], bits, a.D);
+    sv.rows(vt[buf], vp + k0 * a.vs[1], bits, a.D);
   };
   if (t0 < t1) stage(t0, 0);
   for (int t = t0; t < t1; ++t) {
@@ -299,14 +317,13 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
   if (!live) return;
   const long bh = (long)b * a.Hkv + hk;
   if (a.splits > 1) {
-    const long at = ((long)split * a.B * a.Hkv + bh) * a.rows + row;
-    float* po = a.part_o + at * DP;
+    float* po = a.part_o + (((long)split * a.B * a.Hkv + bh) * a.rows + row) * DP;
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         at_store4<float>(po + d * 32 + 8 * i + 4 * h, o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
-    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(base, sum);
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * ((bh * a.rows + row) * a.splits + split)) = make_float2(base, sum);
     return;
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
@@ -325,33 +342,57 @@ __global__ __launch_bounds__(AT_THREADS) void attn_fwd_kernel(AttnArgs a) {
   if (a.stats && h == 0) *reinterpret_cast<float2*>(a.stats + 2 * (bh * a.rows + row)) = make_float2(base == -INFINITY ? 0.f : base, inv);
 }
 
-// joins the key splits: a wave a row;  o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s
-template <typename T>
-__global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a, int DP) {
+// joins the key splits:  o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  WPR waves a row; the lanes of a wave are DP / 4
+// groups of channels times the splits that they add in turn.
+template <typename T, int DP, int WPR>
+__global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
+  constexpr int CG = DP / 4, SG = 64 / CG;      // channel groups, splits a wave adds at a time
+  __shared__ __attribute__((aligned(16))) float red[WPR == 1 ? 1 : AT_WAVES][WPR == 1 ? 4 : DP + 4];
   const long bhs = (long)a.B * a.Hkv, total = bhs * a.rows;
-  const int l = threadIdx.x & 63;
-  const long r = (long)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
-  if (r >= total) return;
+  const int l = threadIdx.x & 63, w = WPR == 1 ? 0 : threadIdx.x >> 6;
+  const long r = (long)blockIdx.x * (AT_WAVES / WPR) + (WPR == 1 ? threadIdx.x >> 6 : 0);
+  if (r >= total) return;                       // (WPR > 1: the whole workgroup)
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + r * a.splits;
   float top = -INFINITY;
-  for (int s = l; s < a.splits; s += 64) top = fmaxf(top, a.part_ml[2 * (s * total + r)]);
+  for (int s = l; s < a.splits; s += 64) top = fmaxf(top, ml[s].x);
   top = wave_max(top);
   const float base = top == -INFINITY ? 0.f : top;
+  const int c = (l % CG) * 4, g = l / CG;
   float sum = 0.f;
-  for (int s = l; s < a.splits; s += 64) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * total + r));
-    sum = fmaf(fast_exp2(ml.x - base), ml.y, sum);
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = w * SG + g; s < a.splits; s += WPR * SG) {
+    const float2 e = ml[s];
+    const float f = fast_exp2(e.x - base);
+    const tapir_f32x4 v = ldg_f4(a.part_o + ((long)s * total + r) * DP + c);
+    sum = fmaf(f, e.y, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fmaf(f, v[i], x[i]);
   }
-  sum = wave_sum(sum);
+#pragma unroll
+  for (int m = CG; m < 64; m <<= 1) {
+    sum += __shfl_xor(sum, m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], m);
+  }
+  if (WPR > 1) {
+    if (g == 0) *reinterpret_cast<float4*>(&red[w][c]) = make_float4(x[0], x[1], x[2], x[3]);
+    if (l == 0) red[w][DP] = sum;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int q = 1; q < WPR; ++q) {
+      sum += red[q][DP];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] += red[q][c + i];
+    }
+  }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   const long bh = r / a.rows, row = r % a.rows, b = bh / a.Hkv, hk = bh % a.Hkv;
   const long at = ((b * a.Nq + row % a.Nq) * a.Hkv * a.G + hk * a.G + row / a.Nq) * a.D;
-  for (int c = l; c < a.D; c += 64) {
-    float x = 0.f;
-    for (int s = 0; s < a.splits; ++s)
-      x = fmaf(fast_exp2(a.part_ml[2 * (s * total + r)] - base), a.part_o[(s * total + r) * DP + c], x);
-    x *= inv;
-    Elem<T>::st((T*)a.out + at + c, x);
-    if (a.out32 && (const void*)a.out32 != a.out) a.out32[at + c] = x;
+  if (g == 0 && c < a.D) {
+    at_store4<T>((T*)a.out + at + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    if (a.out32 && (const void*)a.out32 != a.out) at_store4<float>(a.out32 + at + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
   }
   if (a.stats && l == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(base, inv);
 }
@@ -360,7 +401,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a, int D
 // dq (and D_r on the way): the forward kernel's loop with p from the saved statistics; 1 / l_r is a factor of the whole row and
 // joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip.
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
   __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
@@ -405,12 +446,15 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
   for (int d = 0; d < NB; ++d) o[d] = at_zero();
 
+  AtStage<T, KT, DP> sk, sv;
+  sk.init(a.ks[1]);
+  sv.init(a.vs[1]);
   uint64_t bits = 0;
   auto stage = [&](int t, int buf) {
     const long k0 = (long)t * KT;
     bits = at_key_bits(a, b, k0, len);
-    at_stage<T, KT, DP>(kt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? kp + (k0 + r) * a.ks[1] : (const T*)nullptr; });
-    at_stage<T, KT, DP>(vt[buf], a.D, [&](int r) { return (bits >> r) & 1 ? vp + (k0 + r) * a.vs[1] : (const T*)nullptr; });
+    sk.rows(kt[buf], kp + k0 * a.ks[1], bits, a.D);
+    sv.rows(vt[buf], vp + k0 * a.vs[1], bits, a.D);
   };
   if (t0 < t1) stage(t0, 0);
   for (int t = t0; t < t1; ++t) {
@@ -471,7 +515,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_delta_kernel(AttnArgs a) {
 
 // dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads (or a split of them), RT at a time.
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
   __shared__ __attribute__((aligned(16))) T qt[2][RT * DP];
   __shared__ __attribute__((aligned(16))) T gt[2][RT * DP];
@@ -502,16 +546,37 @@ __global__ __launch_bounds__(AT_THREADS) void attn_dkv_kernel(AttnArgs a) {
   // (a tile behind the clip's length has nothing to add: no steps, zeros are stored)
   const int t0 = split * a.row_steps_per_split, n_steps = kt * AT_KEYS < len ? (int)((a.rows + RT - 1) / RT) : 0;
   const int t1 = n_steps < t0 + a.row_steps_per_split ? n_steps : t0 + a.row_steps_per_split;
+  // a step whose rows belong to one query head takes the same offsets as any other; where heads of fewer than RT queries meet
+  // within a step, each chunk works its own row out
+  typedef AtStage<T, RT, DP> Stage;
+  Stage sq, sg;
+  sq.init(a.qs[1]);
+  sg.init(a.ds[1]);
+  const T* const qb = (const T*)a.q + b * a.qs[0] + (long)hk * a.G * a.qs[2];
+  const T* const gb = (const T*)a.dout + b * a.ds[0] + (long)hk * a.G * a.ds[2];
+  long head0 = 0, query0 = (long)t0 * RT;   // of the next step's first row
+  if (query0 >= a.Nq && t0 < t1) { head0 = query0 / a.Nq; query0 %= a.Nq; }
+  const double per_query = 1.0 / (double)a.Nq;
   auto stage = [&](int t, int buf) {
     const long r0 = (long)t * RT;
-    at_stage<T, RT, DP>(qt[buf], a.D, [&](int r) {
-      const long row = r0 + r;
-      return row < a.rows ? (const T*)a.q + b * a.qs[0] + (row % a.Nq) * a.qs[1] + (hk * a.G + row / a.Nq) * a.qs[2] : (const T*)nullptr;
-    });
-    at_stage<T, RT, DP>(gt[buf], a.D, [&](int r) {
-      const long row = r0 + r;
-      return row < a.rows ? (const T*)a.dout + b * a.ds[0] + (row % a.Nq) * a.ds[1] + (hk * a.G + row / a.Nq) * a.ds[2] : (const T*)nullptr;
-    });
+    const long left = a.rows - r0;
+    if (query0 + RT <= a.Nq || (left < RT && query0 + left <= a.Nq)) {
+      const uint64_t rows = left >= 64 ? ~0ull : (1ull << left) - 1;
+      sq.rows(qt[buf], qb + head0 * a.qs[2] + query0 * a.qs[1], rows, a.D);
+      sg.rows(gt[buf], gb + head0 * a.ds[2] + query0 * a.ds[1], rows, a.D);
+    } else {
+#pragma unroll
+      for (int n = 0; n < Stage::N; ++n) {
+        const int row = (int)r0 + Stage::row(n);
+        // row / Nq: the half keeps the quotient 0.5 / Nq away from whole numbers, far more than its rounding (rows < 2^31)
+        const int head = (int)(((double)row + 0.5) * per_query), query = row - head * (int)a.Nq;
+        const bool ok = row < a.rows && Stage::chunk(n) * EPC < a.D;
+        Stage::put(qt[buf], n, qb + query * a.qs[1] + head * a.qs[2] + Stage::chunk(n) * EPC, ok);
+        Stage::put(gt[buf], n, gb + query * a.ds[1] + head * a.ds[2] + Stage::chunk(n) * EPC, ok);
+      }
+    }
+    query0 += RT;
+    if (query0 >= a.Nq) { head0 += query0 / a.Nq; query0 %= a.Nq; }
     if (threadIdx.x < RT) {
       const long row = r0 + threadIdx.x;
       float2 st = make_float2(0.f, 0.f);
