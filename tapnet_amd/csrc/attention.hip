@@ -150,6 +150,11 @@ int attn_check(tapir_ctx* c, const tapir_attn_args* a, bool backward) {
   auto tensor_ok = [&](const void* p, const int64_t* st, bool empty) {
     return empty || (p && aligned16(p) && st[0] % epc == 0 && st[1] % epc == 0 && st[2] % epc == 0);
   };
+  auto near = [](const int64_t* st) { return st[1] >= 0 && st[1] < AT_MAX_STRIDE; };
+  OP_REQUIRE(c, a->queries <= 1 || (near(a->q_stride) && (!backward || near(a->dout_stride))), TAPIR_ERR_UNSUPPORTED,
+             "cross_attention: tokens of q or dout are 2^22 elements apart or more, or in descending order");
+  OP_REQUIRE(c, a->keys <= 1 || (near(a->k_stride) && near(a->v_stride)), TAPIR_ERR_UNSUPPORTED,
+             "cross_attention: tokens of k or v are 2^22 elements apart or more, or in descending order");
   const bool no_q = a->batch == 0 || a->queries == 0, no_k = a->batch == 0 || a->keys == 0;
   OP_REQUIRE(c, tensor_ok(a->q, a->q_stride, no_q) && tensor_ok(a->k, a->k_stride, no_k) && tensor_ok(a->v, a->v_stride, no_k) &&
                     (!backward || tensor_ok(a->dout, a->dout_stride, no_q)),

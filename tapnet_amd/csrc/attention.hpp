@@ -30,6 +30,7 @@ constexpr int AT_QROWS = 32 * AT_WAVES;      // query rows of a forward / dq wor
 constexpr int AT_KEYS = 32 * AT_WAVES;       // keys of a dk / dv workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float AT_SLACK = 8.f;
+constexpr long AT_MAX_STRIDE = 1L << 22;   // elements from token to token: offsets within a tile of 64 tokens stay below 2^30 bytes
 
 struct AttnArgs {
   const void *q, *k, *v, *dout;
@@ -51,8 +52,6 @@ struct AttnArgs {
   int row_tiles;
   float scale, scale2;                 // scale, scale * log2(e)
 };
-
-__device__ __attribute__((aligned(16))) const unsigned at_zero16[4] = {0u, 0u, 0u, 0u};
 
 // physical 16-byte chunk of logical chunk c in row r of a tile with CH chunks a row: eight consecutive rows reading the same
 // chunk, and four consecutive rows reading a pair of chunks, each touch all banks once.
@@ -92,7 +91,7 @@ __device__ __forceinline__ uint2 at_read_tr(const bf16_t* p) {
 #else
   typedef __attribute__((ext_vector_type(4))) short s16x4;
   typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(uintptr_t)p);
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
   return __builtin_bit_cast(uint2, r);
 #endif
 }
@@ -134,6 +133,14 @@ __device__ __forceinline__ void at_operand(const f32x16& p, float (&w)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = p[i];
 }
+// c plus the 16 values, unrounded: a sum of the rounded ones would make 1 / l_r, and with it every gradient of the row, off by up
+// to a bf16 rounding where one key dominates (two chains: an addition's latency is longer than its issue)
+__device__ __forceinline__ float at_sum(const f32x16& p, float c) {
+  float d = p[0];
+#pragma unroll
+  for (int i = 1; i < 15; i += 2) { c += p[i]; d += p[i + 1]; }
+  return (c + p[15]) + d;
+}
 template <typename T> struct AtOperand;
 template <> struct AtOperand<bf16_t> { unsigned w[8]; };
 template <> struct AtOperand<float> { float w[16]; };
@@ -145,27 +152,48 @@ __device__ __forceinline__ f32x16 at_zero() {
   return z;
 }
 
+// 16 bytes a lane from base + off (base uniform) to LDS, lane i of the wave to `lds` + 16 i; asynchronous: dma_wait().  Written out
+// because the compiler waits for all outstanding copies before every ds_read_b64_tr_b16, whose address it does not analyse: the
+// next tile's copies would then not run under this tile's products.  No register is written, only LDS (M0, the copies' LDS address,
+// serves nothing else in these kernels).
+__device__ __forceinline__ void at_copy16(const void* base, unsigned off, void* lds) {
+#ifdef TAPIR_HIPEMU
+  *((uint4*)lds + (threadIdx.x & 63)) = *(const uint4*)((const char*)base + off);   // (only the lanes that take part)
+#else
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(__builtin_amdgcn_readfirstlane((int)(uintptr_t)lds)), "v"(off), "s"(base) : "memory");
+#endif
+}
+
 // ROWS x DP tile of a [token][channel] tensor -> LDS, 16-byte chunks, by the whole workgroup: thread i copies slots i, i + 256,
 // ... of the tile.  The offsets of a thread's chunks from the tile's first row stay the same for all tiles of a tensor.
 template <typename T, int ROWS, int DP> struct AtStage {
   static constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, N = ROWS * CH / AT_THREADS;
   static_assert(ROWS * CH % AT_THREADS == 0, "tile");
-  long off[N];
+  unsigned off[N];     // bytes (token strides are below AT_MAX_STRIDE elements)
 
   static __device__ __forceinline__ int row(int n) { return (n * AT_THREADS + (int)threadIdx.x) / CH; }
   static __device__ __forceinline__ int chunk(int n) { const int s = n * AT_THREADS + (int)threadIdx.x; return at_swizzle<CH>(s / CH, s % CH); }
   __device__ __forceinline__ void init(long stride) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) off[n] = row(n) * stride + chunk(n) * EPC;
+    for (int n = 0; n < N; ++n) off[n] = (unsigned)((row(n) * stride + chunk(n) * EPC) * (long)sizeof(T));
   }
-  // a chunk from p, or zeros
-  static __device__ __forceinline__ void put(T* lds, int n, const T* p, bool ok) {
-    glds16(ok ? (const void*)p : (const void*)at_zero16, lds + (long)(n * AT_THREADS + (threadIdx.x >> 6) * 64) * EPC);
+  // the thread's n-th chunk from `first` (uniform) + off, or zeros
+  static __device__ __forceinline__ void put(T* lds, int n, const T* first, unsigned off, bool ok) {
+    T* const to = lds + (n * AT_THREADS + (threadIdx.x >> 6) * 64) * EPC;
+    if (ok) at_copy16(first, off, to);
+    else *reinterpret_cast<uint4*>(to + (threadIdx.x & 63) * EPC) = make_uint4(0u, 0u, 0u, 0u);
   }
   // rows from `first` on; row r is zeros where bit r of `bits` is not set, channels from D on are zeros too
   __device__ __forceinline__ void rows(T* lds, const T* first, uint64_t bits, int D) const {
+    constexpr uint64_t all = ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
+    if ((bits & all) == all && D == DP) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) put(lds, n, first + off[n], ((bits >> row(n)) & 1) && chunk(n) * EPC < D);
+      for (int n = 0; n < N; ++n) at_copy16(first, off[n], lds + (n * AT_THREADS + (threadIdx.x >> 6) * 64) * EPC);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) put(lds, n, first, off[n], ((bits >> row(n)) & 1) && chunk(n) * EPC < D);
+    }
   }
 };
 
@@ -173,13 +201,19 @@ template <typename T, int CH> __device__ __forceinline__ uint4 at_chunk(const T*
   return *reinterpret_cast<const uint4*>(X + ((long)r * CH + at_swizzle<CH>(r, c)) * AtFrag<T>::EPC);
 }
 
-// key validity of the 64 keys from k0 as a wave-uniform mask (bit j: key k0 + j takes part)
-__device__ __forceinline__ uint64_t at_key_bits(const AttnArgs& a, int b, long k0, long len) {
-  const long key = k0 + (threadIdx.x & 63);
-  bool ok = key < len;
-  if (a.key_mask != nullptr && ok) ok = a.key_mask[(long)b * a.Nk + key] != 0;
-  return __ballot(ok);
-}
+// Key validity of a tile's keys as a wave-uniform mask (bit j: key k0 + j takes part).  The mask's bytes are read one tile ahead:
+// a load that is waited for here would wait for the copies in flight, too.
+struct AtKeyBits {
+  const unsigned char* mask;     // of the clip, or null
+  long len;
+  unsigned next;                 // the lane's byte of the tile that is staged next
+
+  __device__ __forceinline__ void fetch(long k0) {
+    const long key = k0 + (threadIdx.x & 63);
+    next = mask != nullptr && key < len ? mask[key] : 1;
+  }
+  __device__ __forceinline__ uint64_t bits(long k0) const { return __ballot(k0 + (threadIdx.x & 63) < len && next != 0); }
+};
 
 __device__ __forceinline__ long at_key_len(const AttnArgs& a, int b) {
   if (a.key_lengths == nullptr) return a.Nk;
@@ -256,14 +290,19 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
   AtStage<T, KT, DP> sk, sv;
   sk.init(a.ks[1]);
   sv.init(a.vs[1]);
+  AtKeyBits valid{a.key_mask ? a.key_mask + (long)b * a.Nk : nullptr, len, 1};
   uint64_t bits = 0;
   auto stage = [&](int t, int buf) {
     const long k0 = (long)t * KT;
-    bits = at_key_bits(a, b, k0, len);
+    bits = valid.bits(k0);
     sk.rows(kt[buf], kp + k0 * a.ks[1], bits, a.D);
     sv.rows(vt[buf], vp + k0 * a.vs[1], bits, a.D);
+    valid.fetch(k0 + KT);
   };
+  valid.fetch((long)t0 * KT);
   if (t0 < t1) stage(t0, 0);
+#pragma unroll
+  for (int x = 0; x < CH / 2; ++x) pin(qf[x]);   // (waited for here, not behind the copies of every step)
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const uint64_t cur = bits;
@@ -303,12 +342,10 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -off));
-        sum += s[kb][i];
-      }
+      for (int i = 0; i < 16; ++i) s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -off));
       AtOperand<T> p;
       at_operand(s[kb], p.w);
+      sum = at_sum(s[kb], sum);
 #pragma unroll
       for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], vt[buf], kb * 32, d * 32, p.w);
     }
@@ -440,7 +477,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
     }
   }
   delta += __shfl_xor(delta, 32);
-  const float2 stat = *reinterpret_cast<const float2*>(a.stats + 2 * (bh * a.rows + rr));
+  float row_max = a.stats[2 * (bh * a.rows + rr)], row_inv = a.stats[2 * (bh * a.rows + rr) + 1];
   if (live && h == 0 && split == 0) a.delta[bh * a.rows + row] = delta;
   f32x16 o[NB];
 #pragma unroll
@@ -449,14 +486,21 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
   AtStage<T, KT, DP> sk, sv;
   sk.init(a.ks[1]);
   sv.init(a.vs[1]);
+  AtKeyBits valid{a.key_mask ? a.key_mask + (long)b * a.Nk : nullptr, len, 1};
   uint64_t bits = 0;
   auto stage = [&](int t, int buf) {
     const long k0 = (long)t * KT;
-    bits = at_key_bits(a, b, k0, len);
+    bits = valid.bits(k0);
     sk.rows(kt[buf], kp + k0 * a.ks[1], bits, a.D);
     sv.rows(vt[buf], vp + k0 * a.vs[1], bits, a.D);
+    valid.fetch(k0 + KT);
   };
+  valid.fetch((long)t0 * KT);
   if (t0 < t1) stage(t0, 0);
+#pragma unroll
+  for (int x = 0; x < CH / 2; ++x) { pin(qf[x]); pin(gf[x]); }
+  pin(row_max);
+  pin(row_inv);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const uint64_t cur = bits;
@@ -471,11 +515,13 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
         s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
         g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
       }
-      const unsigned mine = (unsigned)(cur >> (32 * kb)) >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = fast_exp2(fmaf(s[i], a.scale2, -stat.x)) * (g[i] - delta);
-        s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? p : 0.f;
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (g[i] - delta);
+      const unsigned mb = (unsigned)(cur >> (32 * kb));
+      if (mb != 0xffffffffu) {
+        const unsigned mine = mb >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : 0.f;
       }
       AtOperand<T> p;
       at_operand(s, p.w);
@@ -484,7 +530,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
     }
   }
   if (!live) return;
-  const float f = stat.y * a.scale;
+  const float f = row_inv * a.scale;
 #pragma unroll
   for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -519,7 +565,11 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
   __shared__ __attribute__((aligned(16))) T qt[2][RT * DP];
   __shared__ __attribute__((aligned(16))) T gt[2][RT * DP];
-  __shared__ __attribute__((aligned(16))) float ld[2][3][RT];   // m_r, 1 / l_r, D_r
+  // what the rows' products start from and are multiplied by.  bf16: the products begin at -log2(e) L_r / scale2 and -D_r (L_r =
+  // m_r + log l_r), so that p = exp2(scale2 s) and ds = p dp remain; f32: m_r, D_r and 1 / l_r apart, because one number L_r would
+  // be rounded at its own size (2^-21 at 10, a relative error of 5 u of the whole row).
+  constexpr bool BF16 = sizeof(T) == 2;
+  __shared__ __attribute__((aligned(16))) float ld[2][BF16 ? 2 : 3][RT];
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
   const long key_tiles = (a.Nk + AT_KEYS - 1) / AT_KEYS;
   long w = at_work_index();
@@ -548,6 +598,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
   const int t1 = n_steps < t0 + a.row_steps_per_split ? n_steps : t0 + a.row_steps_per_split;
   // a step whose rows belong to one query head takes the same offsets as any other; where heads of fewer than RT queries meet
   // within a step, each chunk works its own row out
+  const float unscale = 1.f / a.scale2;
   typedef AtStage<T, RT, DP> Stage;
   Stage sq, sg;
   sq.init(a.qs[1]);
@@ -557,6 +608,15 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
   long head0 = 0, query0 = (long)t0 * RT;   // of the next step's first row
   if (query0 >= a.Nq && t0 < t1) { head0 = query0 / a.Nq; query0 %= a.Nq; }
   const double per_query = 1.0 / (double)a.Nq;
+  float2 row_stat = make_float2(0.f, 0.f);     // m_r and 1 / l_r, or D_r, of a row of the step that is staged next
+  auto fetch = [&](long r0) {
+    const long row = r0 + (threadIdx.x & (RT - 1));
+    row_stat = make_float2(0.f, 0.f);
+    if (row < a.rows) {
+      if (threadIdx.x < RT) row_stat = *reinterpret_cast<const float2*>(a.stats + 2 * (bh * a.rows + row));
+      else if (threadIdx.x < 2 * RT) row_stat.x = a.delta[bh * a.rows + row];
+    }
+  };
   auto stage = [&](int t, int buf) {
     const long r0 = (long)t * RT;
     const long left = a.rows - r0;
@@ -571,24 +631,28 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         // row / Nq: the half keeps the quotient 0.5 / Nq away from whole numbers, far more than its rounding (rows < 2^31)
         const int head = (int)(((double)row + 0.5) * per_query), query = row - head * (int)a.Nq;
         const bool ok = row < a.rows && Stage::chunk(n) * EPC < a.D;
-        Stage::put(qt[buf], n, qb + query * a.qs[1] + head * a.qs[2] + Stage::chunk(n) * EPC, ok);
-        Stage::put(gt[buf], n, gb + query * a.ds[1] + head * a.ds[2] + Stage::chunk(n) * EPC, ok);
+        const T* const qp = qb + query * a.qs[1] + head * a.qs[2] + Stage::chunk(n) * EPC;
+        const T* const gp = gb + query * a.ds[1] + head * a.ds[2] + Stage::chunk(n) * EPC;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u), qv = ok ? ldg16(qp) : zero, gv = ok ? ldg16(gp) : zero;
+        const int slot = (n * AT_THREADS + (int)threadIdx.x) * EPC;
+        *reinterpret_cast<uint4*>(qt[buf] + slot) = qv;
+        *reinterpret_cast<uint4*>(gt[buf] + slot) = gv;
       }
     }
     query0 += RT;
     if (query0 >= a.Nq) { head0 += query0 / a.Nq; query0 %= a.Nq; }
     if (threadIdx.x < RT) {
-      const long row = r0 + threadIdx.x;
-      float2 st = make_float2(0.f, 0.f);
-      if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + 2 * (bh * a.rows + row));
-      ld[buf][0][threadIdx.x] = st.x;
-      ld[buf][1][threadIdx.x] = st.y;
+      if (BF16) ld[buf][0][threadIdx.x] = (log2f(row_stat.y) - row_stat.x) * unscale;   // (-inf for a row without keys: p = 0)
+      else { ld[buf][0][threadIdx.x] = row_stat.x; ld[buf][BF16 ? 0 : 2][threadIdx.x] = row_stat.y; }
     } else if (threadIdx.x < 2 * RT) {
-      const long row = r0 + (threadIdx.x - RT);
-      ld[buf][2][threadIdx.x - RT] = row < a.rows ? a.delta[bh * a.rows + row] : 0.f;
+      ld[buf][1][threadIdx.x - RT] = BF16 ? -row_stat.x : row_stat.x;
     }
+    fetch(r0 + RT);
   };
+  fetch((long)t0 * RT);
   if (t0 < t1) stage(t0, 0);
+#pragma unroll
+  for (int x = 0; x < CH / 2; ++x) { pin(kf[x]); pin(vf[x]); }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     dma_wait<0>();
@@ -597,22 +661,34 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
 #pragma unroll
     for (int rb = 0; rb < RT; rb += 32) {
       f32x16 s = at_zero(), g = at_zero();
+      if (BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const tapir_f32x4 L = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
+          const tapir_f32x4 E = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { s[4 * i + j] = L[j]; g[4 * i + j] = E[j]; }
+        }
+      }
 #pragma unroll
       for (int x = 0; x < CH / 2; ++x) {
         s = at_mma(at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
         g = at_mma(at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
       }
+      if (BF16) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 M = *reinterpret_cast<const float4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
-        const float4 I = *reinterpret_cast<const float4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
-        const float4 E = *reinterpret_cast<const float4*>(&ld[buf][2][rb + 8 * i + 4 * h]);
-        const float Mv[4] = {M.x, M.y, M.z, M.w}, Iv[4] = {I.x, I.y, I.z, I.w}, Ev[4] = {E.x, E.y, E.z, E.w};
+        for (int i = 0; i < 16; ++i) { s[i] = fast_exp2(s[i] * a.scale2); g[i] *= s[i]; }
+      } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = in ? fast_exp2(fmaf(s[4 * i + j], a.scale2, -Mv[j])) * Iv[j] : 0.f;
-          s[4 * i + j] = p;
-          g[4 * i + j] = p * (g[4 * i + j] - Ev[j]);
+        for (int i = 0; i < 4; ++i) {
+          const tapir_f32x4 M = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
+          const tapir_f32x4 E = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
+          const tapir_f32x4 I = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][BF16 ? 0 : 2][rb + 8 * i + 4 * h]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[4 * i + j] = fast_exp2(fmaf(s[4 * i + j], a.scale2, -M[j])) * I[j];
+            g[4 * i + j] = s[4 * i + j] * (g[4 * i + j] - E[j]);
+          }
         }
       }
       AtOperand<T> p, e;
