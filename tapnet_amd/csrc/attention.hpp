@@ -145,6 +145,20 @@ template <typename T> struct AtOperand;
 template <> struct AtOperand<bf16_t> { unsigned w[8]; };
 template <> struct AtOperand<float> { float w[16]; };
 
+// maximum / sum of the two values that lanes l and l ^ 32 hold
+__device__ __forceinline__ void at_halves(float v, float* a, float* b) {
+#ifdef TAPIR_HIPEMU
+  *a = v;
+  *b = __shfl_xor(v, 32);
+#else
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  *a = __uint_as_float(r[0]);
+  *b = __uint_as_float(r[1]);
+#endif
+}
+__device__ __forceinline__ float at_max_halves(float v) { float a, b; at_halves(v, &a, &b); return fmaxf(a, b); }
+__device__ __forceinline__ float at_sum_halves(float v) { float a, b; at_halves(v, &a, &b); return a + b; }
+
 __device__ __forceinline__ f32x16 at_zero() {
   f32x16 z;
 #pragma unroll
@@ -245,7 +259,7 @@ template <typename T, int DP> struct AtRowTile { static constexpr int RT = 32 * 
 // waves per SIMD that the register allocation aims at
 template <typename T, int DP> struct AtWaves {
   static constexpr bool BF16 = sizeof(T) == 2;
-  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? 3 : (BF16 ? 2 : 1);
+  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? (BF16 ? 4 : 3) : (BF16 ? 2 : 1);
   static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : (BF16 ? 2 : 1);
   static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
 };
@@ -327,7 +341,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
     }
     // The base of the exponentials need not be the running maximum itself: it stays until a score is AT_SLACK powers of two above
     // it (sums and products stay below 2^AT_SLACK per key, far from f32's range), which spares nearly all rescaling of o.
-    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2;
+    top = at_max_halves(top) * a.scale2;
     const bool move = top > base + AT_SLACK;          // (base -inf: every finite score moves it)
     if (__ballot(move) != 0) {
       const float alpha = move ? fast_exp2(base - top) : 1.f;
@@ -350,7 +364,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
       for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], vt[buf], kb * 32, d * 32, p.w);
     }
   }
-  sum += __shfl_xor(sum, 32);
+  sum = at_sum_halves(sum);
   if (!live) return;
   const long bh = (long)b * a.Hkv + hk;
   if (a.splits > 1) {
@@ -476,7 +490,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
       for (int e = 0; e < EPC; ++e) delta = fmaf(Elem<T>::ld(gp + c * EPC + e), a.out32[at + c * EPC + e], delta);
     }
   }
-  delta += __shfl_xor(delta, 32);
+  delta = at_sum_halves(delta);
   float row_max = a.stats[2 * (bh * a.rows + rr)], row_inv = a.stats[2 * (bh * a.rows + rr) + 1];
   if (live && h == 0 && split == 0) a.delta[bh * a.rows + row] = delta;
   f32x16 o[NB];
