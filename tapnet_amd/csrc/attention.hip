@@ -257,7 +257,7 @@ int tapir_layer_norm_workspace(tapir_ctx* c, int64_t rows, int channels, uint64_
   OP_REQUIRE(c, bytes && rows >= 0 && channels >= 1, TAPIR_ERR_INVALID, "layer_norm: bad size");
   const int v = ctx_info(c).dtype == TAPIR_BF16 ? 8 : 4;
   const unsigned shares = std::max(ln_bwd_grid(rows, channels, 1), ln_bwd_grid(rows, channels, v));
-  *bytes = (uint64_t)shares * 2 * channels * sizeof(float);
+  *bytes = (uint64_t)shares * 2 * ln_part_stride(channels) * sizeof(float);
   return TAPIR_OK;
 }
 
@@ -271,7 +271,7 @@ int tapir_layer_norm_backward(tapir_ctx* c, const void* x, int64_t x_stride, con
   const int ept = ln_ept(ci.dtype, channels, x_stride, x, dy_stride, dy, dx);
   const unsigned grid = ln_bwd_grid(rows, channels, ept);
   const bool params = dgamma || dbeta;
-  OP_REQUIRE(c, !params || (workspace && aligned16(workspace) && workspace_bytes >= (uint64_t)grid * 2 * channels * sizeof(float)),
+  OP_REQUIRE(c, !params || (workspace && aligned16(workspace) && workspace_bytes >= (uint64_t)grid * 2 * ln_part_stride(channels) * sizeof(float)),
              TAPIR_ERR_INVALID, "layer_norm: workspace missing or too small (tapir_layer_norm_workspace)");
   OP_TRY(c, hipSetDevice(ci.device));
   const LnBwdArgs a{x, (long)x_stride, dy, (long)dy_stride, gamma, mean, rstd, dx, params ? (float*)workspace : nullptr, (long)rows, channels};
@@ -317,13 +317,40 @@ int tapir_rotary_positions(tapir_ctx* c, const tapir_rotary_args* r, void* strea
   if (r->batch == 0 || r->tokens == 0) return TAPIR_OK;
   OP_REQUIRE(c, r->x && r->y && r->positions, TAPIR_ERR_INVALID, "rotary_positions: null tensor");
   OP_TRY(c, hipSetDevice(ci.device));
+  const int epc = ci.dtype == TAPIR_BF16 ? 8 : 4;
+  const bool bf16 = ci.dtype == TAPIR_BF16;
+  if (r->dim % epc == 0 && r->x_stride[0] % epc == 0 && r->x_stride[1] % epc == 0 && r->x_stride[2] % epc == 0 && aligned16(r->x) &&
+      aligned16(r->y)) {
+    RotaryRowArgs v{};
+    v.x = r->x; v.sb = r->x_stride[0]; v.sn = r->x_stride[1]; v.sh = r->x_stride[2];
+    v.pos = r->positions; v.pb = r->positions_stride; v.y = r->y;
+    v.B = r->batch; v.N = r->tokens; v.H = r->heads; v.D = r->dim; v.axes = r->axes;
+    v.sign = r->inverse ? -1.f : 1.f;
+    for (int i = 0; i < r->dim; ++i) v.other[i] = (unsigned char)i;
+    for (int i = 0; i < pairs; ++i) {
+      v.turns[a.lo[i]] = v.turns[a.hi[i]] = a.turns[i];
+      v.axis[a.lo[i]] = v.axis[a.hi[i]] = a.axis[i];
+      v.other[a.lo[i]] = a.hi[i];
+      v.other[a.hi[i]] = a.lo[i];
+    }
+    const long rpb = (long)(ROT_THREADS / 64) * (64 / (r->dim / epc));   // tokens of a workgroup and step
+    const long base = (r->batch * r->tokens + rpb - 1) / rpb;
+    // few tokens: the heads go to workgroups of their own, ROT_HEADS at most in each, rather than one after the other
+    const int cuts = (int)std::min<long>((r->heads + ROT_HEADS - 1) / ROT_HEADS, std::max<long>(1, 1024 / base));
+    v.heads = (r->heads + cuts - 1) / cuts;
+    const dim3 grid(stride_grid(base), (unsigned)((r->heads + v.heads - 1) / v.heads)), block(ROT_THREADS);
+    if (bf16) hipLaunchKernelGGL((rotary_rows_kernel<bf16_t>), grid, block, 0, (hipStream_t)stream, v);
+    else hipLaunchKernelGGL((rotary_rows_kernel<float>), grid, block, 0, (hipStream_t)stream, v);
+    OP_TRY(c, hipGetLastError());
+    return TAPIR_OK;
+  }
   a.x = r->x; a.sb = r->x_stride[0]; a.sn = r->x_stride[1]; a.sh = r->x_stride[2];
   a.pos = r->positions; a.pb = r->positions_stride; a.y = r->y;
   a.B = r->batch; a.N = r->tokens; a.H = r->heads; a.D = r->dim; a.axes = r->axes; a.pairs = pairs;
   a.sign = r->inverse ? -1.f : 1.f;
   const long work = (a.B * a.N * (a.D - a.pairs) + ROT_THREADS - 1) / ROT_THREADS;
   const dim3 grid(stride_grid(work)), block(ROT_THREADS);
-  if (ci.dtype == TAPIR_BF16) hipLaunchKernelGGL((rotary_kernel<bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+  if (bf16) hipLaunchKernelGGL((rotary_kernel<bf16_t>), grid, block, 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL((rotary_kernel<float>), grid, block, 0, (hipStream_t)stream, a);
   OP_TRY(c, hipGetLastError());
   return TAPIR_OK;

@@ -14,6 +14,9 @@ namespace tapir {
 constexpr int LN_THREADS = 256;
 constexpr int LN_REDUCE_COLS = 16;   // columns per workgroup of the partial sums' reduction
 
+// columns of a row of partial sums: every row starts at a multiple of 16 bytes
+__host__ __device__ __forceinline__ long ln_part_stride(int C) { return ((long)C + 3) & ~3L; }
+
 struct LnArgs {
   const void* x; long ldx;        // [rows, C], row stride in elements
   const float* gamma;             // [C] or null (ones)
@@ -29,24 +32,24 @@ struct LnBwdArgs {
   const float* gamma;
   const float *mean, *rstd;
   void* dx;                       // [rows, C] dense, or null
-  float* part;                    // [grid][2][C] partial sums of dgamma, dbeta (null: neither is wanted)
+  float* part;                    // [grid][2][ln_part_stride(C)] partial sums of dgamma, dbeta (null: neither is wanted)
   long rows; int C;
 };
 
 // EPT consecutive elements at p as floats (EPT * sizeof(T) = 16 bytes, or one element)
 template <typename T, int EPT> struct LnVec;
 template <> struct LnVec<float, 4> {
-  static __device__ __forceinline__ void ld(const float* p, float (&v)[4]) {
-    const tapir_f32x4 r = ldg_f4(p);
-    v[0] = r[0]; v[1] = r[1]; v[2] = r[2]; v[3] = r[3];
-  }
+  typedef tapir_f32x4 Raw;
+  static __device__ __forceinline__ Raw get(const float* p) { return ldg_f4(p); }
+  static __device__ __forceinline__ void split(const Raw& r, float (&v)[4]) { v[0] = r[0]; v[1] = r[1]; v[2] = r[2]; v[3] = r[3]; }
   static __device__ __forceinline__ void st(float* p, const float (&v)[4]) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
 template <> struct LnVec<bf16_t, 8> {
-  static __device__ __forceinline__ void ld(const bf16_t* p, float (&v)[8]) {
-    const uint4 r = ldg16(p);
+  typedef uint4 Raw;
+  static __device__ __forceinline__ Raw get(const bf16_t* p) { return ldg16(p); }
+  static __device__ __forceinline__ void split(const Raw& r, float (&v)[8]) {
     const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
@@ -57,7 +60,9 @@ template <> struct LnVec<bf16_t, 8> {
   }
 };
 template <typename T> struct LnVec<T, 1> {
-  static __device__ __forceinline__ void ld(const T* p, float (&v)[1]) { v[0] = Elem<T>::ld(p); }
+  typedef float Raw;
+  static __device__ __forceinline__ Raw get(const T* p) { return Elem<T>::ld(p); }
+  static __device__ __forceinline__ void split(Raw r, float (&v)[1]) { v[0] = r; }
   static __device__ __forceinline__ void st(T* p, const float (&v)[1]) { Elem<T>::st(p, v[0]); }
 };
 
@@ -89,40 +94,61 @@ __device__ __forceinline__ float ln_block_sum(float v, float* red) {
   return s;
 }
 
-// LPR lanes a row, LN_THREADS / LPR rows a workgroup and step.  C <= LPR * NCH * EPT.
+// a lane's parameters: EPT consecutive columns from `col`, or the value of a missing parameter
+template <int EPT> __device__ __forceinline__ void ln_param(const float* p, int col, int C, float missing, float (&v)[EPT]) {
+  if (EPT >= 4 && p && col < C && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+    for (int e = 0; e < EPT; e += 4) {
+      const tapir_f32x4 r = ldg_f4(p + col + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[EPT >= 4 ? e + i : 0] = r[i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < EPT; ++e) v[e] = p && col < C ? p[col + e] : missing;
+}
+
+// LPR lanes a row, LN_THREADS / LPR rows a workgroup and step; the next step's rows are on their way while this one's are worked on.
+// C <= LPR * NCH * EPT.
 template <typename T, int EPT, int LPR, int NCH>
 __global__ __launch_bounds__(LN_THREADS) void layer_norm_kernel(LnArgs a) {
   constexpr int RPB = LN_THREADS / LPR;
   const int sub = threadIdx.x & (LPR - 1);
+  typename LnVec<T, EPT>::Raw next[NCH];
+  auto fetch = [&](long row0) {
+    const long row = row0 + threadIdx.x / LPR;
+    const T* xp = (const T*)a.x + (row < a.rows ? row : 0) * a.ldx;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * LPR + sub) * EPT;
+      if (col < a.C) next[c] = LnVec<T, EPT>::get(xp + col);
+    }
+  };
+  const long first = (long)blockIdx.x * RPB, step = (long)gridDim.x * RPB;
+  if (first < a.rows) fetch(first);
   float gm[NCH][EPT], bt[NCH][EPT];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
-    const int col = (c * LPR + sub) * EPT;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      gm[c][e] = a.gamma && col < a.C ? a.gamma[col + e] : 1.f;
-      bt[c][e] = a.beta && col < a.C ? a.beta[col + e] : 0.f;
-    }
+    ln_param(a.gamma, (c * LPR + sub) * EPT, a.C, 1.f, gm[c]);
+    ln_param(a.beta, (c * LPR + sub) * EPT, a.C, 0.f, bt[c]);
   }
   const float inv = 1.f / (float)a.C;
-  for (long row0 = (long)blockIdx.x * RPB; row0 < a.rows; row0 += (long)gridDim.x * RPB) {
+  for (long row0 = first; row0 < a.rows; row0 += step) {
     const long row = row0 + threadIdx.x / LPR;
-    const bool live = row < a.rows;
-    const T* xp = (const T*)a.x + (live ? row : 0) * a.ldx;
     float x[NCH][EPT];
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * LPR + sub) * EPT;
-      if (col < a.C) {
-        LnVec<T, EPT>::ld(xp + col, x[c]);
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) x[c][e] = 0.f;
+      if ((c * LPR + sub) * EPT < a.C) {
+        LnVec<T, EPT>::split(next[c], x[c]);
 #pragma unroll
         for (int e = 0; e < EPT; ++e) s += x[c][e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) x[c][e] = 0.f;
       }
     }
+    if (row0 + step < a.rows) fetch(row0 + step);
     const float mean = ln_sum<LPR>(s) * inv;
     float ss = 0.f;
 #pragma unroll
@@ -132,7 +158,7 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_kernel(LnArgs a) {
         for (int e = 0; e < EPT; ++e) { x[c][e] -= mean; ss = fmaf(x[c][e], x[c][e], ss); }
       }
     const float rstd = 1.f / sqrtf(ln_sum<LPR>(ss) * inv + a.eps);
-    if (!live) continue;
+    if (row >= a.rows) continue;
     T* yp = (T*)a.y + row * a.C;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -180,24 +206,38 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_kernel(LnBwdArgs a)
   for (int c = 0; c < NCH; ++c) {
     const int col = (c * LPR + sub) * EPT;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) { gm[c][e] = a.gamma && col < a.C ? a.gamma[col + e] : 1.f; dg[c][e] = 0.f; db[c][e] = 0.f; }
+    for (int e = 0; e < EPT; ++e) { dg[c][e] = 0.f; db[c][e] = 0.f; }
+    ln_param(a.gamma, col, a.C, 1.f, gm[c]);
   }
   const float inv = 1.f / (float)a.C;
-  for (long row0 = (long)blockIdx.x * RPB; row0 < a.rows; row0 += (long)gridDim.x * RPB) {
+  typename LnVec<T, EPT>::Raw nx[NCH], ny[NCH];
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](long row0) {
+    const long row = row0 + threadIdx.x / LPR, r = row < a.rows ? row : 0;
+    nmean = a.mean[r];
+    nrstd = a.rstd[r];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * LPR + sub) * EPT;
+      if (col < a.C) {
+        nx[c] = LnVec<T, EPT>::get((const T*)a.x + r * a.ldx + col);
+        ny[c] = LnVec<T, EPT>::get((const T*)a.dy + r * a.lddy + col);
+      }
+    }
+  };
+  const long first = (long)blockIdx.x * RPB, step = (long)gridDim.x * RPB;
+  if (first < a.rows) fetch(first);
+  for (long row0 = first; row0 < a.rows; row0 += step) {
     const long row = row0 + threadIdx.x / LPR;
     const bool live = row < a.rows;
-    const long r = live ? row : 0;
-    const T* xp = (const T*)a.x + r * a.ldx;
-    const T* yp = (const T*)a.dy + r * a.lddy;
-    const float mean = a.mean[r], rstd = a.rstd[r];
+    const float mean = nmean, rstd = nrstd;
     float u[NCH][EPT], g[NCH][EPT];
     float sg = 0.f, su = 0.f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * LPR + sub) * EPT;
-      if (live && col < a.C) {
-        LnVec<T, EPT>::ld(xp + col, u[c]);
-        LnVec<T, EPT>::ld(yp + col, g[c]);
+      if (live && (c * LPR + sub) * EPT < a.C) {
+        LnVec<T, EPT>::split(nx[c], u[c]);
+        LnVec<T, EPT>::split(ny[c], g[c]);
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
           u[c][e] = (u[c][e] - mean) * rstd;
@@ -209,6 +249,7 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_kernel(LnBwdArgs a)
         }
       }
     }
+    if (row0 + step < a.rows) fetch(row0 + step);
     sg = ln_sum<LPR>(sg) * inv;
     su = ln_sum<LPR>(su) * inv;
     if (!live || !a.dx) continue;
@@ -225,7 +266,8 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_kernel(LnBwdArgs a)
     }
   }
   if (!a.part) return;
-  float* part = a.part + (long)blockIdx.x * 2 * a.C;
+  const long ps = ln_part_stride(a.C);
+  float* part = a.part + (long)blockIdx.x * 2 * ps;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
 #pragma unroll
@@ -239,7 +281,7 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_kernel(LnBwdArgs a)
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < RPB; ++q) s += red[q * LPR * EPT + k];
-        if (col < a.C) part[(long)which * a.C + col] = s;
+        if (col < a.C) part[which * ps + col] = s;
       }
     }
   }
@@ -250,9 +292,10 @@ template <typename T>
 __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_long_kernel(LnBwdArgs a) {
   __shared__ float red[LN_THREADS / 64];
   const float inv = 1.f / (float)a.C;
-  float* part = a.part ? a.part + (long)blockIdx.x * 2 * a.C : nullptr;
+  const long ps = ln_part_stride(a.C);
+  float* part = a.part ? a.part + (long)blockIdx.x * 2 * ps : nullptr;
   if (part)
-    for (int c = threadIdx.x; c < a.C; c += LN_THREADS) { part[c] = 0.f; part[a.C + c] = 0.f; }
+    for (int c = threadIdx.x; c < a.C; c += LN_THREADS) { part[c] = 0.f; part[ps + c] = 0.f; }
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* xp = (const T*)a.x + row * a.ldx;
     const T* yp = (const T*)a.dy + row * a.lddy;
@@ -262,7 +305,7 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_long_kernel(LnBwdAr
       const float dy = Elem<T>::ld(yp + c), u = (Elem<T>::ld(xp + c) - mean) * rstd, g = a.gamma ? dy * a.gamma[c] : dy;
       sg += g;
       su = fmaf(g, u, su);
-      if (part) { part[c] = fmaf(dy, u, part[c]); part[a.C + c] += dy; }   // (a column belongs to one thread)
+      if (part) { part[c] = fmaf(dy, u, part[c]); part[ps + c] += dy; }   // (a column belongs to one thread)
     }
     sg = ln_block_sum(sg, red) * inv;
     su = ln_block_sum(su, red) * inv;
@@ -275,24 +318,38 @@ __global__ __launch_bounds__(LN_THREADS) void layer_norm_bwd_long_kernel(LnBwdAr
   }
 }
 
-// dgamma / dbeta = the sum of the workgroups' shares, LN_REDUCE_COLS columns a workgroup, its rows of threads striding the shares
+// dgamma / dbeta = the sum of the workgroups' shares: LN_REDUCE_COLS columns a workgroup, four of them a thread, 64 rows of threads
+// striding the shares (512 shares: eight loads a thread, in flight together).  Columns up to the padded stride are read and dropped.
 __global__ __launch_bounds__(LN_THREADS) inline void layer_norm_reduce_kernel(const float* part, int shares, int C, float* dgamma,
                                                                               float* dbeta) {
-  constexpr int RW = LN_THREADS / LN_REDUCE_COLS;
-  __shared__ float red[LN_THREADS];
+  constexpr int CQ = LN_REDUCE_COLS / 4, RW = LN_THREADS / CQ;
+  __shared__ __attribute__((aligned(16))) float red[LN_THREADS * 4];
   float* out = blockIdx.y ? dbeta : dgamma;
   if (!out) return;
-  const int k = threadIdx.x % LN_REDUCE_COLS, r = threadIdx.x / LN_REDUCE_COLS;
-  const int col = blockIdx.x * LN_REDUCE_COLS + k;
-  float s = 0.f;
-  if (col < C)
-    for (int p = r; p < shares; p += RW) s += part[((long)p * 2 + blockIdx.y) * C + col];
-  red[threadIdx.x] = s;
-  __syncthreads();
-  if (r == 0 && col < C) {
+  const int k = threadIdx.x % CQ, r = threadIdx.x / CQ;
+  const long ps = ln_part_stride(C), col = (long)blockIdx.x * LN_REDUCE_COLS + 4 * k;
+  tapir_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (col < ps) {
+#pragma unroll 8
+    for (int p = r; p < shares; p += RW) s += ldg_f4(part + ((long)p * 2 + blockIdx.y) * ps + col);
+  }
 #pragma unroll
-    for (int q = 1; q < RW; ++q) s += red[q * LN_REDUCE_COLS + k];
-    out[col] = s;
+  for (int i = 0; i < 4; ++i) red[r * LN_REDUCE_COLS + 4 * k + i] = s[i];
+  __syncthreads();
+  // 256 threads: 16 a column, then one
+  const int q = threadIdx.x / LN_REDUCE_COLS, j = threadIdx.x % LN_REDUCE_COLS;
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < RW / (LN_THREADS / LN_REDUCE_COLS); ++i) v += red[(q * (RW / (LN_THREADS / LN_REDUCE_COLS)) + i) * LN_REDUCE_COLS + j];
+  __syncthreads();
+  red[threadIdx.x] = v;
+  __syncthreads();
+  const long c = (long)blockIdx.x * LN_REDUCE_COLS + threadIdx.x;
+  if (threadIdx.x < LN_REDUCE_COLS && c < C) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < LN_THREADS / LN_REDUCE_COLS; ++i) t += red[i * LN_REDUCE_COLS + threadIdx.x];
+    out[c] = t;
   }
 }
 
