@@ -86,7 +86,7 @@ void ln_bwd_dispatch(const LnBwdArgs& a, unsigned grid, hipStream_t s) {
 
 // ---------------------------------------------------------------------------------------------------- attention
 int attn_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
-int attn_row_step(int dtype, int dp) { return 32L * dp * (dtype == TAPIR_BF16 ? 2 : 4) / 16 >= AT_THREADS ? 32 : 64; }   // AtRowTile
+int attn_row_step(int dtype, int dp) { return dtype != TAPIR_BF16 && dp > 32 ? 32 : 64; }   // AtRowTile
 
 struct AttnPlan {
   int dp, row_tiles, splits, tiles_per_split, row_splits, row_steps_per_split;

@@ -246,8 +246,9 @@ template <> __device__ __forceinline__ void at_store4<bf16_t>(bf16_t* p, float x
 
 // keys a forward / dq step stages: 64 (bf16) or 32 (f32)
 template <typename T> struct AtTile { static constexpr int KT = sizeof(T) == 2 ? 64 : 32; };
-// query rows a dk / dv step stages: 32, or 64 where 32 rows are less than a copy per thread
-template <typename T, int DP> struct AtRowTile { static constexpr int RT = 32 * DP * (int)sizeof(T) / 16 >= AT_THREADS ? 32 : 64; };
+// query rows a dk / dv step stages: 64, so that the next step's copies have two blocks of products to arrive under (bf16, 64
+// channels: 256 x 49152 x 4 x 64: 60 -> 51 us); f32, whose products take eight times as long: 32 where that is a copy per thread
+template <typename T, int DP> struct AtRowTile { static constexpr int RT = sizeof(T) == 4 && DP > 32 ? 32 : 64; };
 
 // ------------------------------------------------------------------------------------------------------- work distribution
 // splits of a clip's keys that hold any (at least one: it writes the zeros of a clip without tokens)
