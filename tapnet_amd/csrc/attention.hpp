@@ -98,19 +98,26 @@ __device__ __forceinline__ uint2 at_read_tr(const bf16_t* p) {
 
 // c[32 channels from d0][32 columns] += X[32 summed rows from r0][channels]^T * w, w = 16 values a lane in the layout of a
 // 32 x 32 product (register i of lane half h: summed row 8 (i / 4) + 4 h + i % 4).  X: a tile of CH-chunk rows in LDS.
+struct AtTr { uint2 t[4]; };     // a lane's share of X's 32 rows from r0, 32 channels from d0
+template <int CH> __device__ __forceinline__ AtTr at_tr(const bf16_t* X, int r0, int d0) {
+  const int l = threadIdx.x & 63, h = l >> 5, i = l & 15;
+  AtTr x;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = r0 + 8 * u + 4 * h + (i >> 2), col = d0 + (l & 16) + 4 * (i & 3);
+    x.t[u] = at_read_tr(X + ((long)r * CH + at_swizzle<CH>(r, col >> 3)) * 8 + (col & 7));
+  }
+  return x;
+}
+__device__ __forceinline__ void at_mma_tr(f32x16& c, const AtTr& x, const unsigned (&w)[8]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    c = at_mma(make_uint4(x.t[2 * s].x, x.t[2 * s].y, x.t[2 * s + 1].x, x.t[2 * s + 1].y),
+               make_uint4(w[4 * s], w[4 * s + 1], w[4 * s + 2], w[4 * s + 3]), c, bf16_t{});
+}
 template <int CH>
 __device__ __forceinline__ void at_mma_tr(f32x16& c, const bf16_t* X, int r0, int d0, const unsigned (&w)[8]) {
-  const int l = threadIdx.x & 63, h = l >> 5, i = l & 15;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    uint2 t[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = r0 + 16 * s + 8 * u + 4 * h + (i >> 2), col = d0 + (l & 16) + 4 * (i & 3);
-      t[u] = at_read_tr(X + ((long)r * CH + at_swizzle<CH>(r, col >> 3)) * 8 + (col & 7));
-    }
-    c = at_mma(make_uint4(t[0].x, t[0].y, t[1].x, t[1].y), make_uint4(w[4 * s], w[4 * s + 1], w[4 * s + 2], w[4 * s + 3]), c, bf16_t{});
-  }
+  at_mma_tr(c, at_tr<CH>(X, r0, d0), w);
 }
 template <int CH>
 __device__ __forceinline__ void at_mma_tr(f32x16& c, const float* X, int r0, int d0, const float (&w)[16]) {
@@ -263,76 +270,75 @@ __device__ __forceinline__ long at_clip_key_tiles(const AttnArgs& a, int b) { re
 // keys (rows) that neighbouring units share.  Only units that hold work are counted (`active` of them): clips of different lengths
 // would otherwise leave whole dies idle (3 clips of 8200, 4100 and 0 tokens: 489 -> 290 us a training step).  Returns the unit, or
 // -1 - i for the i-th workgroup that is left over.
-__device__ __forceinline__ long at_unit(long active) {
-  const long n = gridDim.x, i = blockIdx.x, x = i % 8, j = i / 8;
-  const long q = active / 8, r = active % 8, mine = q + (x < r);
-  if (j < mine) return x * q + (x < r ? x : r) + j;
-  const long nq = n / 8, nr = n % 8;
-  return -1 - (x * (nq - q) + (x < nr ? x : nr) - (x < r ? x : r) + j - mine);
+__device__ __forceinline__ int at_unit(unsigned active) {
+  const unsigned n = gridDim.x, i = blockIdx.x, x = i % 8, j = i / 8;
+  const unsigned q = active / 8, r = active % 8, mine = q + (x < r);
+  if (j < mine) return (int)(x * q + (x < r ? x : r) + j);
+  const unsigned nq = n / 8, nr = n % 8;
+  return -1 - (int)(x * (nq - q) + (x < nr ? x : nr) - (x < r ? x : r) + j - mine);
 }
 
-struct AtUnit { int b, hk, split; long tile; };
+struct AtUnit { int b, hk, split, tile; };
+
+// (units fit 31 bits: 64-bit divisions of them took a third of a short workgroup's prologue)
+__device__ __forceinline__ AtUnit at_decode(int b, unsigned w, unsigned tiles, unsigned splits) {
+  const unsigned rest = w / tiles, hk = rest / splits;
+  return AtUnit{b, (int)hk, (int)(rest - hk * splits), (int)(w - rest * tiles)};
+}
 
 // forward / dq: units ordered by clip, key head, split of the keys, row tile
 template <typename T> __device__ __forceinline__ bool at_row_unit(const AttnArgs& a, AtUnit* u) {
-  const long per = (long)a.Hkv * a.row_tiles;
-  long w;
-  int splits = a.splits, b = 0;
+  const unsigned per = (unsigned)(a.Hkv * a.row_tiles);
+  unsigned w, splits = a.splits;
+  int b = 0;
   if (a.key_lengths == nullptr) {
     w = at_unit(gridDim.x);
     b = (int)(w / (per * splits));
     w -= b * per * splits;
   } else {
-    long active = 0;
+    unsigned active = 0;
     for (int c = 0; c < a.B; ++c) active += per * at_clip_splits<T>(a, c);
-    w = at_unit(active);
-    if (w < 0) return false;
+    const int i = at_unit(active);
+    if (i < 0) return false;
+    w = i;
     for (;; ++b) {
       splits = at_clip_splits<T>(a, b);
       if (w < per * splits) break;
       w -= per * splits;
     }
   }
-  const long rest = w / a.row_tiles;
-  *u = AtUnit{b, (int)(rest / splits), (int)(rest % splits), w - rest * a.row_tiles};
+  *u = at_decode(b, w, a.row_tiles, splits);
   return true;
 }
 
 // dk / dv: units ordered by clip, key head, split of the rows, key tile.  Tiles behind a clip's length come back from the workgroups
 // that are left over, as `zero`: there is nothing to sum, but dk and dv are to be written.
 __device__ __forceinline__ bool at_key_unit(const AttnArgs& a, AtUnit* u, bool* zero) {
-  const long tiles = (a.Nk + AT_KEYS - 1) / AT_KEYS, per = (long)a.Hkv * a.row_splits;
+  const unsigned tiles = (unsigned)((a.Nk + AT_KEYS - 1) / AT_KEYS), per = (unsigned)(a.Hkv * a.row_splits);
   *zero = false;
-  long w, n = tiles, first = 0;
-  int b = 0, splits = a.row_splits;
+  unsigned w, n = tiles, first = 0;
+  int b = 0;
   if (a.key_lengths == nullptr) {
     w = at_unit(gridDim.x);
     b = (int)(w / (per * tiles));
     w -= b * per * tiles;
   } else {
-    long active = 0;
-    for (int c = 0; c < a.B; ++c) active += per * at_clip_key_tiles(a, c);
-    w = at_unit(active);
-    if (w >= 0) {
-      for (;; ++b) {
-        n = at_clip_key_tiles(a, b);
-        if (w < per * n) break;
-        w -= per * n;
-      }
-    } else {
-      if (a.row_splits > 1) return false;     // (the join writes the zeros)
-      *zero = true;
-      w = -1 - w;
-      for (;; ++b) {
-        first = at_clip_key_tiles(a, b);
-        n = tiles - first;
-        if (w < per * n) break;
-        w -= per * n;
-      }
+    unsigned active = 0;
+    for (int c = 0; c < a.B; ++c) active += per * (unsigned)at_clip_key_tiles(a, c);
+    const int i = at_unit(active);
+    if (i < 0 && a.row_splits > 1) return false;     // (the join writes the zeros)
+    *zero = i < 0;
+    w = i < 0 ? -1 - i : i;
+    for (;; ++b) {
+      const unsigned full = (unsigned)at_clip_key_tiles(a, b);
+      first = i < 0 ? full : 0;
+      n = i < 0 ? tiles - full : full;
+      if (w < per * n) break;
+      w -= per * n;
     }
   }
-  const long rest = w / n;
-  *u = AtUnit{b, (int)(rest / splits), (int)(rest % splits), first + w - rest * n};
+  *u = at_decode(b, w, n, a.row_splits);
+  u->tile += first;
   return true;
 }
 
@@ -356,11 +362,11 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
   AtUnit unit;
   if (!at_row_unit<T>(a, &unit)) return;
   const int b = unit.b, hk = unit.hk, split = unit.split;
-  const long row = unit.tile * AT_QROWS + wave * 32 + (l & 31);
+  const unsigned row = (unsigned)(unit.tile * AT_QROWS + wave * 32 + (l & 31));
   const bool live = row < a.rows;
-  const long rr = live ? row : 0;
-  const int head = hk * a.G + (int)(rr / a.Nq);
-  const long query = rr % a.Nq;
+  const unsigned rr = live ? row : 0, in_group = rr / (unsigned)a.Nq;
+  const int head = hk * a.G + (int)in_group;
+  const long query = rr - in_group * (unsigned)a.Nq;
   const long len = at_key_len(a, b);
   const int t0 = split * a.tiles_per_split;
   const long n_tiles = (len + KT - 1) / KT;
@@ -533,6 +539,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
 // joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
+  constexpr bool AHEAD = false;
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
   __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
@@ -540,11 +547,11 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
   AtUnit unit;
   if (!at_row_unit<T>(a, &unit)) return;
   const int b = unit.b, hk = unit.hk, split = unit.split;
-  const long row = unit.tile * AT_QROWS + wave * 32 + (l & 31);
+  const unsigned row = (unsigned)(unit.tile * AT_QROWS + wave * 32 + (l & 31));
   const bool live = row < a.rows;
-  const long rr = live ? row : 0;
-  const int head = hk * a.G + (int)(rr / a.Nq);
-  const long query = rr % a.Nq;
+  const unsigned rr = live ? row : 0, in_group = rr / (unsigned)a.Nq;
+  const int head = hk * a.G + (int)in_group;
+  const long query = rr - in_group * (unsigned)a.Nq;
   const long len = at_key_len(a, b);
   const int t0 = split * a.tiles_per_split;
   const long n_tiles = (len + KT - 1) / KT;
@@ -600,13 +607,35 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
     dma_wait<0>();
     __syncthreads();
     if (t + 1 < t1) stage(t + 1, buf ^ 1);
+    uint4 ka[CH / 2], va[CH / 2];
+    auto read = [&](int kb) {
+#pragma unroll
+      for (int x = 0; x < CH / 2; ++x) {
+        ka[x] = at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h);
+        va[x] = at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h);
+      }
+    };
+    if constexpr (AHEAD) read(0);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       f32x16 s = at_zero(), g = at_zero();
+      AtTr kx[NB];
+      if constexpr (AHEAD) {
 #pragma unroll
-      for (int x = 0; x < CH / 2; ++x) {
-        s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
-        g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
+        for (int x = 0; x < CH / 2; ++x) {
+          s = at_mma(ka[x], qf[x], s, T{});
+          g = at_mma(va[x], gf[x], g, T{});
+        }
+#pragma unroll
+        for (int d = 0; d < NB; ++d) kx[d] = at_tr<CH>(kt[buf], kb * 32, d * 32);
+        if (kb + 1 < KT / 32) read(kb + 1);
+        sched_fence();
+      } else {
+#pragma unroll
+        for (int x = 0; x < CH / 2; ++x) {
+          s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
+          g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (g[i] - delta);
@@ -619,7 +648,10 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
       AtOperand<T> p;
       at_operand(s, p.w);
 #pragma unroll
-      for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], kt[buf], kb * 32, d * 32, p.w);
+      for (int d = 0; d < NB; ++d) {
+        if constexpr (AHEAD) at_mma_tr(o[d], kx[d], p.w);
+        else at_mma_tr<CH>(o[d], kt[buf], kb * 32, d * 32, p.w);
+      }
     }
   }
   if (!live) return;
@@ -668,8 +700,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
   bool zero;
   if (!at_key_unit(a, &unit, &zero)) return;
   const int b = unit.b, hk = unit.hk, split = unit.split;
-  const long kt = unit.tile;
-  const long key = kt * AT_KEYS + wave * 32 + (l & 31);
+  const int kt = unit.tile;
+  const long key = (long)kt * AT_KEYS + wave * 32 + (l & 31);
   const long len = at_key_len(a, b);
   bool in = key < len;
   if (in && a.key_mask != nullptr) in = a.key_mask[(long)b * a.Nk + key] != 0;
@@ -697,32 +729,42 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
   sg.init(a.ds[1]);
   const T* const qb = (const T*)a.q + b * a.qs[0] + (long)hk * a.G * a.qs[2];
   const T* const gb = (const T*)a.dout + b * a.ds[0] + (long)hk * a.G * a.ds[2];
-  long head0 = 0, query0 = (long)t0 * RT;   // of the next step's first row
-  if (query0 >= a.Nq && t0 < t1) { head0 = query0 / a.Nq; query0 %= a.Nq; }
+  const int Nq = (int)a.Nq, n_rows = (int)a.rows;
+  int head0 = 0, query0 = t0 * RT;   // of the next step's first row
+  if (query0 >= Nq && t0 < t1) { head0 = (unsigned)query0 / (unsigned)Nq; query0 -= head0 * Nq; }
   const double per_query = 1.0 / (double)a.Nq;
   float2 row_stat = make_float2(0.f, 0.f);     // m_r and 1 / l_r, or D_r, of a row of the step that is staged next
-  auto fetch = [&](long r0) {
-    const long row = r0 + (threadIdx.x & (RT - 1));
+  const float* const row_stats = a.stats + 2 * bh * a.rows;
+  const float* const row_delta = a.delta + bh * a.rows;
+  auto fetch = [&](int r0) {
+    const int row = r0 + (int)(threadIdx.x & (RT - 1));
     row_stat = make_float2(0.f, 0.f);
-    if (row < a.rows) {
-      if (threadIdx.x < RT) row_stat = *reinterpret_cast<const float2*>(a.stats + 2 * (bh * a.rows + row));
-      else if (threadIdx.x < 2 * RT) row_stat.x = a.delta[bh * a.rows + row];
+    if (row < n_rows) {
+      if (threadIdx.x < RT) row_stat = *reinterpret_cast<const float2*>(row_stats + 2 * (long)row);
+      else if (threadIdx.x < 2 * RT) row_stat.x = row_delta[row];
     }
   };
-  auto stage = [&](int t, int buf) {
-    const long r0 = (long)t * RT;
-    const long left = a.rows - r0;
-    if (query0 + RT <= a.Nq || (left < RT && query0 + left <= a.Nq)) {
+  auto put_stats = [&](int buf) {
+    if (threadIdx.x < RT) {
+      if (BF16) ld[buf][0][threadIdx.x] = (log2f(row_stat.y) - row_stat.x) * unscale;   // (-inf for a row without keys: p = 0)
+      else { ld[buf][0][threadIdx.x] = row_stat.x; ld[buf][BF16 ? 0 : 2][threadIdx.x] = row_stat.y; }
+    } else if (threadIdx.x < 2 * RT) {
+      ld[buf][1][threadIdx.x - RT] = BF16 ? -row_stat.x : row_stat.x;
+    }
+  };
+  auto copy = [&](int t, int buf) {
+    const int r0 = t * RT, left = n_rows - r0;
+    if (query0 + RT <= Nq || (left < RT && query0 + left <= Nq)) {
       const uint64_t rows = left >= 64 ? ~0ull : (1ull << left) - 1;
       sq.rows(qt[buf], qb + head0 * a.qs[2] + query0 * a.qs[1], rows, a.D);
       sg.rows(gt[buf], gb + head0 * a.ds[2] + query0 * a.ds[1], rows, a.D);
     } else {
 #pragma unroll
       for (int n = 0; n < Stage::N; ++n) {
-        const int row = (int)r0 + Stage::row(n);
+        const int row = r0 + Stage::row(n);
         // row / Nq: the half keeps the quotient 0.5 / Nq away from whole numbers, far more than its rounding (rows < 2^31)
-        const int head = (int)(((double)row + 0.5) * per_query), query = row - head * (int)a.Nq;
-        const bool ok = row < a.rows && Stage::chunk(n) * EPC < a.D;
+        const int head = (int)(((double)row + 0.5) * per_query), query = row - head * Nq;
+        const bool ok = row < n_rows && Stage::chunk(n) * EPC < a.D;
         const T* const qp = qb + query * a.qs[1] + head * a.qs[2] + Stage::chunk(n) * EPC;
         const T* const gp = gb + query * a.ds[1] + head * a.ds[2] + Stage::chunk(n) * EPC;
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u), qv = ok ? ldg16(qp) : zero, gv = ok ? ldg16(gp) : zero;
@@ -732,28 +774,40 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
       }
     }
     query0 += RT;
-    if (query0 >= a.Nq) { head0 += query0 / a.Nq; query0 %= a.Nq; }
-    if (threadIdx.x < RT) {
-      if (BF16) ld[buf][0][threadIdx.x] = (log2f(row_stat.y) - row_stat.x) * unscale;   // (-inf for a row without keys: p = 0)
-      else { ld[buf][0][threadIdx.x] = row_stat.x; ld[buf][BF16 ? 0 : 2][threadIdx.x] = row_stat.y; }
-    } else if (threadIdx.x < 2 * RT) {
-      ld[buf][1][threadIdx.x - RT] = BF16 ? -row_stat.x : row_stat.x;
-    }
-    fetch(r0 + RT);
+    if (query0 >= Nq) { const int more = (unsigned)query0 / (unsigned)Nq; head0 += more; query0 -= more * Nq; }
   };
-  fetch((long)t0 * RT);
-  if (t0 < t1) stage(t0, 0);
+  if (t0 < t1) {
+    fetch(t0 * RT);
+    copy(t0, 0);
+    put_stats(0);
+    fetch((t0 + 1) * RT);
+  }
 #pragma unroll
   for (int x = 0; x < CH / 2; ++x) { pin(kf[x]); pin(vf[x]); }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     dma_wait<0>();
     __syncthreads();
-    if (t + 1 < t1) stage(t + 1, buf ^ 1);
+    if (t + 1 < t1) {
+      put_stats(buf ^ 1);         // (waits for the statistics: before the copies are under way)
+      copy(t + 1, buf ^ 1);
+      fetch((t + 2) * RT);
+    }
+    if constexpr (BF16) {
+      // Operands are read from LDS a phase before the products that take them, and the fences keep it so: left to itself the
+      // compiler reads each right before its product and waits (2 x 1000 x 8200 x 2 x 128: XX us)
+      uint4 qa[CH / 2], ga[CH / 2];
+      auto read = [&](int rb) {
 #pragma unroll
-    for (int rb = 0; rb < RT; rb += 32) {
-      f32x16 s = at_zero(), g = at_zero();
-      if (BF16) {
+        for (int x = 0; x < CH / 2; ++x) {
+          qa[x] = at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h);
+          ga[x] = at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h);
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int rb = 0; rb < RT; rb += 32) {
+        f32x16 s, g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const tapir_f32x4 L = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
@@ -761,35 +815,59 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
 #pragma unroll
           for (int j = 0; j < 4; ++j) { s[4 * i + j] = L[j]; g[4 * i + j] = E[j]; }
         }
-      }
+        AtTr gx[NB], qx[NB];
 #pragma unroll
-      for (int x = 0; x < CH / 2; ++x) {
-        s = at_mma(at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
-        g = at_mma(at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
-      }
-      if (BF16) {
+        for (int d = 0; d < NB; ++d) gx[d] = at_tr<CH>(gt[buf], rb, d * 32);
+        sched_fence();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = fast_exp2(s[i] * a.scale2); g[i] *= s[i]; }
-      } else {
+        for (int x = 0; x < CH / 2; ++x) {
+          s = at_mma(qa[x], kf[x], s, T{});
+          g = at_mma(ga[x], vf[x], g, T{});
+        }
+#pragma unroll
+        for (int d = 0; d < NB; ++d) qx[d] = at_tr<CH>(qt[buf], rb, d * 32);
+        if (rb + 32 < RT) read(rb + 32);
+        sched_fence();
+        AtOperand<T> p, e;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = fast_exp2(s[i] * a.scale2);
+        at_operand(s, p.w);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) at_mma_tr(dv[d], gx[d], p.w);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[i] *= s[i];
+        at_operand(g, e.w);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) at_mma_tr(dk[d], qx[d], e.w);
+      }
+    } else {
+#pragma unroll
+      for (int rb = 0; rb < RT; rb += 32) {
+        f32x16 s = at_zero(), g = at_zero();
+#pragma unroll
+        for (int x = 0; x < CH / 2; ++x) {
+          s = at_mma(at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
+          g = at_mma(at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const tapir_f32x4 M = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
           const tapir_f32x4 E = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
-          const tapir_f32x4 I = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][BF16 ? 0 : 2][rb + 8 * i + 4 * h]);
+          const tapir_f32x4 I = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][2][rb + 8 * i + 4 * h]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             s[4 * i + j] = fast_exp2(fmaf(s[4 * i + j], a.scale2, -M[j])) * I[j];
             g[4 * i + j] = s[4 * i + j] * (g[4 * i + j] - E[j]);
           }
         }
-      }
-      AtOperand<T> p, e;
-      at_operand(s, p.w);
-      at_operand(g, e.w);
+        AtOperand<T> p, e;
+        at_operand(s, p.w);
+        at_operand(g, e.w);
 #pragma unroll
-      for (int d = 0; d < NB; ++d) {
-        at_mma_tr<CH>(dv[d], gt[buf], rb, d * 32, p.w);
-        at_mma_tr<CH>(dk[d], qt[buf], rb, d * 32, e.w);
+        for (int d = 0; d < NB; ++d) {
+          at_mma_tr<CH>(dv[d], gt[buf], rb, d * 32, p.w);
+          at_mma_tr<CH>(dk[d], qt[buf], rb, d * 32, e.w);
+        }
       }
     }
   }
