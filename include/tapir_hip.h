@@ -443,7 +443,8 @@ int tapir_rotary_positions(tapir_ctx* ctx, const tapir_rotary_args* args, void* 
  * `out` itself) and stats [batch, kv_heads, heads / kv_heads * queries, 2] are written.
  * The backward pass takes the forward call's arguments (out may be NULL), dout (strides like q's) and writes dq and dk,
  * dv, dense (dq, or dk and dv together, may be NULL); rows of dk / dv outside the masks are zeros.  kv heads shared by
- * several query heads receive their sum.  The workspace call for it is made with dq, dk and dv set. */
+ * several query heads receive their sum.  The workspace calls take the same arguments
+ * as the calls that they are for. */
 typedef struct tapir_attn_args {
   int64_t batch, queries, keys;
   int heads, kv_heads, dim;

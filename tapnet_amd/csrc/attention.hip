@@ -95,24 +95,48 @@ struct AttnPlan {
 
 size_t round4(size_t n) { return (n + 3) & ~(size_t)3; }   // (shares of a workspace start at multiples of 16 bytes)
 
-// Splits of a long axis: where the tiles of the other one alone leave compute units idle (`base` workgroups), it is cut until
-// there are `want`, each of `least` steps at least (the join reads a partial result per split).
-void attn_split(long steps, long base, long want, long least, int* splits, int* per) {
-  long s = std::min<long>((want + base - 1) / base, (steps + least - 1) / least);
-  s = std::max<long>(1, std::min<long>(s, 1024));
-  *per = (int)((steps + s - 1) / s);
-  *splits = (int)((steps + *per - 1) / *per);
+// Splits of a long axis: `base` workgroups of `steps` steps each become base * s of steps / s, joined at `join` us a split.  The s of
+// the least estimated time is taken.  Estimate: n workgroups that share a compute unit (of 256) take t1 max(1 + (n - 1) / 2, 0.7 n)
+// a step (4096 queries x 49152 keys x 64, forward: 0.92, 1.37, 1.93, 2.55 us for 1 to 4), `occupancy` of them at once, and three
+// steps' time to begin.  Measured, 256 x 49152 x 4 x 64: forward 699 us unsplit, 34 / 30 / 32 / 34 / 39 us for 256 / 512 / 768 / 1024 /
+// 1536 workgroups; 3 x 1000 x 8200 x 2 x 128: backward 169 us with the rows of dk / dv unsplit, 189 / 202 / 224 us with 2 / 3 / 6 splits.
+struct AttnSplit { long steps, base; int occupancy; double t1, join, join_first; };
+void attn_split(const AttnSplit& x, int* splits, int* per_split) {
+  double best = 0;
+  *splits = 0;
+  auto shared = [&](long n) { return n == 0 ? 0.0 : x.t1 * std::max(1 + 0.5 * (n - 1), 0.7 * n); };
+  for (long s = 1, per = x.steps;; ) {
+    const long n = (x.base * s + 255) / 256, full = n / x.occupancy;
+    const double t = (per + 3) * (full * shared(x.occupancy) + shared(n % x.occupancy)) + (s > 1 ? x.join_first + x.join * s : 0);
+    if (*splits == 0 || t < best) { best = t; *splits = (int)s; *per_split = (int)per; }
+    if (per == 1 || n > 2 * x.occupancy) break;
+    --per;                                        // the next number of splits that shortens them
+    s = (x.steps + per - 1) / per;
+    per = (x.steps + s - 1) / s;
+    if (s > 1024) break;
+  }
 }
 
 AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
   AttnPlan p{};
   const bool bf16 = dtype == TAPIR_BF16;
   p.dp = attn_pad(a->dim);
+  const int w = p.dp == 32 ? 0 : p.dp == 64 ? 1 : 2;
   const long rows = (long)(a->heads / a->kv_heads) * a->queries, heads = std::max<long>(1, (long)a->batch * a->kv_heads);
   p.row_tiles = (int)((rows + AT_QROWS - 1) / AT_QROWS);
   const int kt = bf16 ? 64 : 32;
   const long tiles = std::max<long>(1, (a->keys + kt - 1) / kt);
-  attn_split(tiles, std::max<long>(1, heads * p.row_tiles), backward ? 512 : 1024, 4, &p.splits, &p.tiles_per_split);
+  const double us_per_byte = 1 / 9e6;   // partial results, mostly out of the last-level cache
+  // us a step of a workgroup that has its compute unit to itself, and workgroups a compute unit holds (AtWaves)
+  static const double fwd_us[2][3] = {{1.3, 2.6, 5.0}, {0.65, 0.92, 1.7}}, dq_us[2][3] = {{1.9, 3.6, 7.0}, {0.8, 1.2, 2.4}};
+  static const double dkv_us[2][3] = {{5.0, 5.0, 10.0}, {0.9, 1.4, 2.4}};
+  static const int fwd_occ[2][3] = {{4, 3, 1}, {4, 4, 2}}, dq_occ[2][3] = {{4, 2, 1}, {4, 3, 2}}, dkv_occ[2][3] = {{2, 2, 1}, {3, 2, 1}};
+  const double row_bytes = 8.0 * heads * rows * p.dp, key_bytes = 16.0 * heads * a->keys * p.dp;   // written and read
+  // (a padded batch is taken to hold two thirds of its tokens: the lengths themselves are on the device)
+  auto filled = [&](long units) { return std::max<long>(1, a->key_lengths ? units * 2 / 3 : units); };
+  const AttnSplit keys{tiles, filled(heads * p.row_tiles), backward ? dq_occ[bf16][w] : fwd_occ[bf16][w],
+                       backward ? dq_us[bf16][w] : fwd_us[bf16][w], row_bytes * us_per_byte, backward ? 3.0 : 4.0};
+  attn_split(keys, &p.splits, &p.tiles_per_split);
   if (!backward) {
     if (p.splits > 1) {
       const size_t r = (size_t)p.splits * a->batch * a->kv_heads * rows;
@@ -122,8 +146,9 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
     return p;
   }
   const int rt = attn_row_step(dtype, p.dp);
-  attn_split(std::max<long>(1, (rows + rt - 1) / rt), std::max<long>(1, heads * ((a->keys + AT_KEYS - 1) / AT_KEYS)), 512, 4,
-             &p.row_splits, &p.row_steps_per_split);
+  const AttnSplit by_row{std::max<long>(1, (rows + rt - 1) / rt), filled(heads * ((a->keys + AT_KEYS - 1) / AT_KEYS)),
+                         dkv_occ[bf16][w], dkv_us[bf16][w], key_bytes * us_per_byte, p.splits > 1 ? 1.0 : 3.0};
+  attn_split(by_row, &p.row_splits, &p.row_steps_per_split);
   p.delta = round4((size_t)heads * rows);
   if (p.splits > 1 && a->dq) p.part_dq = (size_t)p.splits * a->batch * a->queries * a->heads * a->dim;
   if (p.row_splits > 1 && a->dk) p.part_dkv = (size_t)p.row_splits * a->batch * a->keys * a->kv_heads * a->dim;
