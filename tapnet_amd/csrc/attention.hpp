@@ -140,6 +140,18 @@ __device__ __forceinline__ void at_operand(const f32x16& p, float (&w)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = p[i];
 }
+// The same in two parts, w + v: the 16 most significant bits and the bf16 of what is left (2^-16 together).  ds takes this way: it has
+// either sign, its products with k and q cancel in part, and one rounding of it made dq and dk up to 1.7 times as far off as their own
+// final rounding does (p, all positive, is rounded once: 1.4 times for dv).
+__device__ __forceinline__ void at_operand2(const f32x16& p, unsigned (&w)[8], unsigned (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned a = __float_as_uint(p[2 * i]) & 0xffff0000u, b = __float_as_uint(p[2 * i + 1]) & 0xffff0000u;
+    w[i] = (a >> 16) | b;
+    v[i] = pack_bf16x2(p[2 * i] - __uint_as_float(a), p[2 * i + 1] - __uint_as_float(b));
+  }
+}
+
 // c plus the 16 values, unrounded: a sum of the rounded ones would make 1 / l_r, and with it every gradient of the row, off by up
 // to a bf16 rounding where one key dominates (two chains: an addition's latency is longer than its issue)
 __device__ __forceinline__ float at_sum(const f32x16& p, float c) {
@@ -539,7 +551,6 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
 // joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
-  constexpr bool AHEAD = false;
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
   __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
@@ -607,35 +618,13 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
     dma_wait<0>();
     __syncthreads();
     if (t + 1 < t1) stage(t + 1, buf ^ 1);
-    uint4 ka[CH / 2], va[CH / 2];
-    auto read = [&](int kb) {
-#pragma unroll
-      for (int x = 0; x < CH / 2; ++x) {
-        ka[x] = at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h);
-        va[x] = at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h);
-      }
-    };
-    if constexpr (AHEAD) read(0);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       f32x16 s = at_zero(), g = at_zero();
-      AtTr kx[NB];
-      if constexpr (AHEAD) {
 #pragma unroll
-        for (int x = 0; x < CH / 2; ++x) {
-          s = at_mma(ka[x], qf[x], s, T{});
-          g = at_mma(va[x], gf[x], g, T{});
-        }
-#pragma unroll
-        for (int d = 0; d < NB; ++d) kx[d] = at_tr<CH>(kt[buf], kb * 32, d * 32);
-        if (kb + 1 < KT / 32) read(kb + 1);
-        sched_fence();
-      } else {
-#pragma unroll
-        for (int x = 0; x < CH / 2; ++x) {
-          s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
-          g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
-        }
+      for (int x = 0; x < CH / 2; ++x) {
+        s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
+        g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (g[i] - delta);
@@ -645,12 +634,20 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : 0.f;
       }
-      AtOperand<T> p;
-      at_operand(s, p.w);
+      if constexpr (sizeof(T) == 2) {
+        unsigned w[8], v[8];
+        at_operand2(s, w, v);
 #pragma unroll
-      for (int d = 0; d < NB; ++d) {
-        if constexpr (AHEAD) at_mma_tr(o[d], kx[d], p.w);
-        else at_mma_tr<CH>(o[d], kt[buf], kb * 32, d * 32, p.w);
+        for (int d = 0; d < NB; ++d) {
+          const AtTr x = at_tr<CH>(kt[buf], kb * 32, d * 32);
+          at_mma_tr(o[d], x, w);
+          at_mma_tr(o[d], x, v);
+        }
+      } else {
+        AtOperand<T> p;
+        at_operand(s, p.w);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], kt[buf], kb * 32, d * 32, p.w);
       }
     }
   }
@@ -836,9 +833,12 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         for (int d = 0; d < NB; ++d) at_mma_tr(dv[d], gx[d], p.w);
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[i] *= s[i];
-        at_operand(g, e.w);
+        AtOperand<T> f;
+        at_operand2(g, e.w, f.w);
 #pragma unroll
         for (int d = 0; d < NB; ++d) at_mma_tr(dk[d], qx[d], e.w);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) at_mma_tr(dk[d], qx[d], f.w);
       }
     } else {
 #pragma unroll
