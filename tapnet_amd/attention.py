@@ -9,8 +9,10 @@ bfloat16; sums, statistics and the parameters of a norm are float32 in both.
 
 Calls are enqueued on the current stream of the tensors' device, whatever the current device is; nothing synchronises.
 Scratch memory comes from torch's allocator, so calls on several streams and captured graphs do not share any.  A graph
-may capture them once a call of the same element type has been made on the device (it prepares the library).  No kernel uses
-atomics: the same call gives the same bits.  Gradients are not differentiable again.
+may capture them once a call of the same element type has been made on the device (it prepares the library); a backward
+pass is captured on a side stream, with no eager autograd graph of the same leaves alive (torch's autograd engine would
+wait for the eager graph's stream inside the capture).  No kernel uses atomics: the same call gives the same bits, also where
+only some of the gradients are asked for.  Gradients are not differentiable again.
 
 The argument checks and autograd nodes are in ``csrc/torch_ops.cpp`` (built beside the library).
 """
@@ -77,5 +79,5 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
   ``dim ** -0.5``.
 
   Returns ``[batch, queries, heads, dim]`` in q's type.  Scores, statistics and sums are float32; in bfloat16 the
-  probabilities (and in the gradient the scores' gradients) are rounded to bfloat16 on their way into the second product."""
+  forward pass rounds the probabilities to bfloat16 on their way into the second product (the gradients keep 16 bits of them)."""
   return _ops().cross_attention(q, k, v, key_lengths, key_mask, scale)

@@ -236,7 +236,7 @@ void attn_bwd_launch(const AttnArgs& k, hipStream_t s) {
     hipLaunchKernelGGL((attn_dq_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
   } else if (k.rows > 0) {
     const long rows = (long)k.B * k.Hkv * k.rows;
-    hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k);
+    hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 32 * AT_WAVES - 1) / (32 * AT_WAVES))), dim3(AT_THREADS), 0, s, k);
   }
   if (k.Nk > 0 && k.dk) {
     const unsigned grid = (unsigned)((long)k.B * k.Hkv * ((k.Nk + AT_KEYS - 1) / AT_KEYS) * k.row_splits);

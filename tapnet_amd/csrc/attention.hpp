@@ -130,8 +130,8 @@ __device__ __forceinline__ void at_mma_tr(f32x16& c, const float* X, int r0, int
   }
 }
 
-// the 16 values of a lane as the operand of at_mma_tr: rounded to bf16 (the products of the next sum take bf16 operands; the
-// relative error of each term, 2^-8 at most, is the size of the output's own rounding and averages out over the sum), or as they are
+// the 16 values of a lane as the operand of at_mma_tr: as they are (f32), or rounded to bf16.  The forward pass rounds p once: its
+// weights of one sign add up, the error (2^-8 a term at most, a third of that on average) stays near the output's own rounding.
 __device__ __forceinline__ void at_operand(const f32x16& p, unsigned (&w)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
@@ -140,9 +140,9 @@ __device__ __forceinline__ void at_operand(const f32x16& p, float (&w)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = p[i];
 }
-// The same in two parts, w + v: the 16 most significant bits and the bf16 of what is left (2^-16 together).  ds takes this way: it has
-// either sign, its products with k and q cancel in part, and one rounding of it made dq and dk up to 1.7 times as far off as their own
-// final rounding does (p, all positive, is rounded once: 1.4 times for dv).
+// The same in two parts, w + v: the 16 most significant bits and the bf16 of what is left (2^-16 together).  The gradients take this
+// way: their terms have either sign and cancel in part, and with one rounding of ds and p the gradients were 1.45 to 1.7 times as far
+// from the exact ones as their own final rounding is (256 queries x 49152 keys: 6 us of 95 for p, 10 us for ds).
 __device__ __forceinline__ void at_operand2(const f32x16& p, unsigned (&w)[8], unsigned (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -188,12 +188,12 @@ __device__ __forceinline__ f32x16 at_zero() {
 // 16 bytes a lane from base + off (base uniform) to LDS, lane i of the wave to `lds` + 16 i; asynchronous: dma_wait().  Written out
 // because the compiler waits for all outstanding copies before every ds_read_b64_tr_b16, whose address it does not analyse: the
 // next tile's copies would then not run under this tile's products.  No register is written, only LDS (M0, the copies' LDS address,
-// serves nothing else in these kernels).
+// serves nothing else in these kernels).  The wait covers M0 and a base that a vector instruction wrote into scalar registers just before.
 __device__ __forceinline__ void at_copy16(const void* base, unsigned off, void* lds) {
 #ifdef TAPIR_HIPEMU
   *((uint4*)lds + (threadIdx.x & 63)) = *(const uint4*)((const char*)base + off);   // (only the lanes that take part)
 #else
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(__builtin_amdgcn_readfirstlane((int)(uintptr_t)lds)), "v"(off), "s"(base) : "memory");
 #endif
 }
@@ -270,17 +270,17 @@ template <typename T> struct AtTile { static constexpr int KT = sizeof(T) == 2 ?
 template <typename T, int DP> struct AtRowTile { static constexpr int RT = sizeof(T) == 4 && DP > 32 ? 32 : 64; };
 
 // ------------------------------------------------------------------------------------------------------- work distribution
-// splits of a clip's keys that hold any (at least one: it writes the zeros of a clip without tokens)
-template <typename T> __device__ __forceinline__ int at_clip_splits(const AttnArgs& a, int b) {
+// splits of a clip's keys that hold any (at least one: it writes the zeros of a clip without tokens); its key tiles that do
+template <typename T> __device__ __forceinline__ unsigned at_clip_splits(const AttnArgs& a, int b) {
   if (a.key_lengths == nullptr) return a.splits;
-  const long step = (long)a.tiles_per_split * AtTile<T>::KT, n = (at_key_len(a, b) + step - 1) / step;
-  return n < 1 ? 1 : (int)n;
+  const unsigned tiles = (unsigned)((at_key_len(a, b) + AtTile<T>::KT - 1) / AtTile<T>::KT), per = a.tiles_per_split;
+  return tiles <= per ? 1 : (tiles + per - 1) / per;
 }
-__device__ __forceinline__ long at_clip_key_tiles(const AttnArgs& a, int b) { return (at_key_len(a, b) + AT_KEYS - 1) / AT_KEYS; }
+__device__ __forceinline__ unsigned at_clip_key_tiles(const AttnArgs& a, int b) { return (unsigned)((at_key_len(a, b) + AT_KEYS - 1) / AT_KEYS); }
 
 // Workgroups are dealt to the 8 dies in turn; each die takes one run of consecutive units of work, so that its own L2 serves the
 // keys (rows) that neighbouring units share.  Only units that hold work are counted (`active` of them): clips of different lengths
-// would otherwise leave whole dies idle (3 clips of 8200, 4100 and 0 tokens: 489 -> 290 us a training step).  Returns the unit, or
+// would otherwise leave whole dies idle (3 clips of 8200, 4100 and 0 tokens: 489 -> 291 us a training step).  Returns the unit, or
 // -1 - i for the i-th workgroup that is left over.
 __device__ __forceinline__ int at_unit(unsigned active) {
   const unsigned n = gridDim.x, i = blockIdx.x, x = i % 8, j = i / 8;
@@ -292,6 +292,43 @@ __device__ __forceinline__ int at_unit(unsigned active) {
 
 struct AtUnit { int b, hk, split, tile; };
 
+__device__ __forceinline__ unsigned at_uniform(unsigned v) { return (unsigned)__builtin_amdgcn_readfirstlane((int)v); }
+
+// Units of all clips, count(clip) each: 64 clips at a time, a lane each
+template <class F> __device__ __forceinline__ unsigned at_units(int B, const F& count) {
+  unsigned total = 0;
+  for (int c = 0; c < B; c += 64) {
+    const int clip = c + (int)(threadIdx.x & 63);
+    unsigned v = clip < B ? count(clip) : 0;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += (unsigned)__shfl_xor((int)v, m);
+    total += at_uniform(v);
+  }
+  return total;
+}
+// the clip that unit w of them falls to; w becomes its index within the clip, n the clip's count
+template <class F> __device__ __forceinline__ int at_find_clip(int B, const F& count, unsigned* w, unsigned* n) {
+  const int l = threadIdx.x & 63;
+  for (int c = 0; c < B; c += 64) {
+    const unsigned v = c + l < B ? count(c + l) : 0;
+    unsigned upto = v;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const unsigned before = (unsigned)__shfl((int)upto, (l - m) & 63);
+      if (l >= m) upto += before;
+    }
+    const uint64_t behind = __ballot(upto > *w);
+    if (behind != 0) {
+      const int lane = (int)at_uniform((unsigned)__builtin_ctzll(behind));
+      *n = at_uniform((unsigned)__shfl((int)v, lane));
+      *w -= at_uniform((unsigned)__shfl((int)upto, lane)) - *n;
+      return c + lane;
+    }
+    *w -= at_uniform((unsigned)__shfl((int)upto, 63));
+  }
+  return 0;   // (not reached: w is below the sum)
+}
+
 // (units fit 31 bits: 64-bit divisions of them took a third of a short workgroup's prologue)
 __device__ __forceinline__ AtUnit at_decode(int b, unsigned w, unsigned tiles, unsigned splits) {
   const unsigned rest = w / tiles, hk = rest / splits;
@@ -302,22 +339,18 @@ __device__ __forceinline__ AtUnit at_decode(int b, unsigned w, unsigned tiles, u
 template <typename T> __device__ __forceinline__ bool at_row_unit(const AttnArgs& a, AtUnit* u) {
   const unsigned per = (unsigned)(a.Hkv * a.row_tiles);
   unsigned w, splits = a.splits;
-  int b = 0;
+  int b;
   if (a.key_lengths == nullptr) {
     w = at_unit(gridDim.x);
     b = (int)(w / (per * splits));
     w -= b * per * splits;
   } else {
-    unsigned active = 0;
-    for (int c = 0; c < a.B; ++c) active += per * at_clip_splits<T>(a, c);
-    const int i = at_unit(active);
+    auto count = [&](int clip) { return per * at_clip_splits<T>(a, clip); };
+    const int i = at_unit(at_units(a.B, count));
     if (i < 0) return false;
     w = i;
-    for (;; ++b) {
-      splits = at_clip_splits<T>(a, b);
-      if (w < per * splits) break;
-      w -= per * splits;
-    }
+    b = at_find_clip(a.B, count, &w, &splits);
+    splits /= per;
   }
   *u = at_decode(b, w, a.row_tiles, splits);
   return true;
@@ -329,25 +362,21 @@ __device__ __forceinline__ bool at_key_unit(const AttnArgs& a, AtUnit* u, bool* 
   const unsigned tiles = (unsigned)((a.Nk + AT_KEYS - 1) / AT_KEYS), per = (unsigned)(a.Hkv * a.row_splits);
   *zero = false;
   unsigned w, n = tiles, first = 0;
-  int b = 0;
+  int b;
   if (a.key_lengths == nullptr) {
     w = at_unit(gridDim.x);
     b = (int)(w / (per * tiles));
     w -= b * per * tiles;
   } else {
-    unsigned active = 0;
-    for (int c = 0; c < a.B; ++c) active += per * (unsigned)at_clip_key_tiles(a, c);
-    const int i = at_unit(active);
+    auto count = [&](int clip) { return per * at_clip_key_tiles(a, clip); };
+    const int i = at_unit(at_units(a.B, count));
     if (i < 0 && a.row_splits > 1) return false;     // (the join writes the zeros)
     *zero = i < 0;
     w = i < 0 ? -1 - i : i;
-    for (;; ++b) {
-      const unsigned full = (unsigned)at_clip_key_tiles(a, b);
-      first = i < 0 ? full : 0;
-      n = i < 0 ? tiles - full : full;
-      if (w < per * n) break;
-      w -= per * n;
-    }
+    if (i < 0) b = at_find_clip(a.B, [&](int clip) { return per * (tiles - at_clip_key_tiles(a, clip)); }, &w, &n);
+    else b = at_find_clip(a.B, count, &w, &n);
+    n /= per;
+    first = i < 0 ? tiles - n : 0;
   }
   *u = at_decode(b, w, n, a.row_splits);
   u->tile += first;
@@ -552,6 +581,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
+  constexpr bool BF16 = sizeof(T) == 2;
   __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
@@ -597,6 +627,9 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
   AtStage<T, KT, DP> sk, sv;
   sk.init(a.ks[1]);
   sv.init(a.vs[1]);
+  f32x16 minus_delta;      // bf16: what the products with dout begin at
+#pragma unroll
+  for (int i = 0; i < 16; ++i) minus_delta[i] = -delta;
   AtKeyBits valid{a.key_mask ? a.key_mask + (long)b * a.Nk : nullptr, len, 1};
   uint64_t bits = 0;
   auto stage = [&](int t, int buf) {
@@ -620,21 +653,21 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
     if (t + 1 < t1) stage(t + 1, buf ^ 1);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
-      f32x16 s = at_zero(), g = at_zero();
+      f32x16 s = at_zero(), g = BF16 ? minus_delta : at_zero();
 #pragma unroll
       for (int x = 0; x < CH / 2; ++x) {
         s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
         g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (g[i] - delta);
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (BF16 ? g[i] : g[i] - delta);
       const unsigned mb = (unsigned)(cur >> (32 * kb));
       if (mb != 0xffffffffu) {
         const unsigned mine = mb >> (4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : 0.f;
       }
-      if constexpr (sizeof(T) == 2) {
+      if constexpr (BF16) {
         unsigned w[8], v[8];
         at_operand2(s, w, v);
 #pragma unroll
@@ -666,19 +699,22 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
     }
 }
 
-// D_r where dq is not wanted: a wave a row
+// D_r where dq is not wanted: two lanes a row, the sums in the order of attn_dq_kernel
 template <typename T>
 __global__ __launch_bounds__(AT_THREADS) void attn_delta_kernel(AttnArgs a) {
-  const long total = (long)a.B * a.Hkv * a.rows, r = (long)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
-  if (r >= total) return;
+  constexpr int EPC = AtFrag<T>::EPC;
   const int l = threadIdx.x & 63;
-  const long bh = r / a.rows, row = r % a.rows, b = bh / a.Hkv, head = bh % a.Hkv * a.G + row / a.Nq, query = row % a.Nq;
+  const long total = (long)a.B * a.Hkv * a.rows, r = ((long)blockIdx.x * AT_WAVES + (threadIdx.x >> 6)) * 32 + (l & 31);
+  const bool live = r < total;
+  const long rr = live ? r : 0, bh = rr / a.rows, row = rr % a.rows, b = bh / a.Hkv, head = bh % a.Hkv * a.G + row / a.Nq, query = row % a.Nq;
   const T* gp = (const T*)a.dout + b * a.ds[0] + query * a.ds[1] + head * a.ds[2];
   const float* op = a.out32 + ((b * a.Nq + query) * a.Hkv * a.G + head) * a.D;
   float delta = 0.f;
-  for (int c = l; c < a.D; c += 64) delta = fmaf(Elem<T>::ld(gp + c), op[c], delta);
-  delta = wave_sum(delta);
-  if (l == 0) a.delta[r] = delta;
+  for (int c = l >> 5; live && c * EPC < a.D; c += 2)
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) delta = fmaf(Elem<T>::ld(gp + c * EPC + e), op[c * EPC + e], delta);
+  delta = at_sum_halves(delta);
+  if (live && l < 32) a.delta[r] = delta;
 }
 
 // dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads (or a split of them), RT at a time.
@@ -825,15 +861,16 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         for (int d = 0; d < NB; ++d) qx[d] = at_tr<CH>(qt[buf], rb, d * 32);
         if (rb + 32 < RT) read(rb + 32);
         sched_fence();
-        AtOperand<T> p, e;
+        AtOperand<T> p, e, f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = fast_exp2(s[i] * a.scale2);
-        at_operand(s, p.w);
+        at_operand2(s, p.w, f.w);
 #pragma unroll
         for (int d = 0; d < NB; ++d) at_mma_tr(dv[d], gx[d], p.w);
 #pragma unroll
+        for (int d = 0; d < NB; ++d) at_mma_tr(dv[d], gx[d], f.w);
+#pragma unroll
         for (int i = 0; i < 16; ++i) g[i] *= s[i];
-        AtOperand<T> f;
         at_operand2(g, e.w, f.w);
 #pragma unroll
         for (int d = 0; d < NB; ++d) at_mma_tr(dk[d], qx[d], e.w);

@@ -99,6 +99,8 @@ Tensor workspace(uint64_t bytes, const Tensor& like) {
 // Gradients are not differentiable again: asked for a second derivative, the node behind them says so.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g.set_requires_grad(true);
   auto node = std::make_shared<torch::autograd::DelayedError>(
       "the operators of tapnet_amd.attention have no second derivative", static_cast<int64_t>(grads.size()));
   return (*node)(std::move(grads));
@@ -294,12 +296,14 @@ Tensor rotary_positions(const Tensor& x, const Tensor& positions_, const std::op
 }
 
 // ----------------------------------------------------------------------------------------------------- cross attention
-// `t` itself where its rows (last axis) are dense and start at multiples of 16 bytes, else a dense copy
+// `t` itself where its rows (last axis) are dense, start at multiples of 16 bytes and are less than 2^22 elements apart, else a
+// dense copy
 Tensor aligned(const Tensor& in) {
   Tensor t = plain(in);
   const int64_t epc = 16 / static_cast<int64_t>(t.element_size());
   bool good = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int d = 0; d < 3; ++d) good = good && t.stride(d) % epc == 0;
+  good = good && (t.size(1) <= 1 || t.stride(1) < (int64_t{1} << 22));
   if (good) return t;
   t = t.contiguous();
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);

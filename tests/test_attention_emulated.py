@@ -157,7 +157,7 @@ def attn_args(q, k, v, lengths=None, mask=None, scale=None):
   return a
 
 
-def run_attention(c, q, k, v, lengths=None, mask=None, scale=None, dout=None):
+def run_attention(c, q, k, v, lengths=None, mask=None, scale=None, dout=None, wanted='qkv'):
   a = attn_args(q, k, v, lengths, mask, scale)
   out = aligned_empty(q.shape, q.dtype)
   a.out = out.data_ptr()
@@ -173,7 +173,7 @@ def run_attention(c, q, k, v, lengths=None, mask=None, scale=None, dout=None):
     return [out]
   a.dout, a.dout_stride[:] = dout.data_ptr(), dout.stride()[:3]
   grads = [aligned_empty(t.shape, t.dtype) for t in (q, k, v)]
-  a.dq, a.dk, a.dv = (g.data_ptr() for g in grads)
+  a.dq, a.dk, a.dv = (g.data_ptr() if n in wanted else None for n, g in zip('qkv', grads))
   c('tapir_cross_attention_workspace', ctypes.byref(a), 1, ctypes.byref(nbytes))
   work = workspace(nbytes.value)
   a.workspace, a.workspace_bytes = work.data_ptr(), nbytes.value
@@ -241,6 +241,55 @@ def test_cross_attention_masks(dtype, how):
   empty = ~keep.any(1)
   assert empty.any() and (got[0][empty] == 0).all() and (got[1][empty] == 0).all()
   assert (got[2][~keep] == 0).all() and (got[3][~keep] == 0).all()
+
+
+@pytest.mark.parametrize('queries,keys', [(3, 300), (400, 200), (70, 1500)])
+def test_cross_attention_many_clips(queries, keys):
+  """More clips than a wave has lanes, of all lengths from none to whole: each is found, and what nobody sums is zero."""
+  batch, heads, kv_heads, dim = 70 if keys < 1000 else 9, 1, 1, 8
+  gen = torch.Generator().manual_seed(13)
+  q, k, v, dout = inputs(gen, torch.bfloat16, batch, queries, keys, heads, kv_heads, dim)
+  lengths = torch.randint(0, keys + 1, (batch,), generator=gen).to(torch.int32)
+  lengths[0], lengths[1], lengths[-1], lengths[-2] = 0, keys, keys, 0
+  with Ctx(torch.bfloat16) as c:
+    got = run_attention(c, q, k, v, lengths, dout=dout)
+  want = R.attention(q, k, v, keep_mask(batch, keys, lengths, None), dim ** -0.5, dout)
+  for name, g, w in zip(('out', 'dq', 'dk', 'dv'), got, want):
+    R.check(name, g, w)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('queries,keys', [(5, 90), (300, 40)])
+def test_cross_attention_some_gradients(dtype, queries, keys):
+  """dq alone and dk / dv alone give the bits of the whole backward pass."""
+  gen = torch.Generator().manual_seed(14)
+  q, k, v, dout = inputs(gen, dtype, 2, queries, keys, 4, 2, 24)
+  lengths = torch.tensor([keys, 7], dtype=torch.int32)
+  with Ctx(dtype) as c:
+    whole = run_attention(c, q, k, v, lengths, dout=dout)
+    for wanted in ('q', 'kv'):
+      part = run_attention(c, q, k, v, lengths, dout=dout, wanted=wanted)
+      for n, (g, w) in enumerate(zip(part[1:], whole[1:])):
+        if 'qkv'[n] in wanted:
+          assert torch.equal(g, w)
+        else:
+          assert torch.isnan(g.float()).all()    # not written
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_cross_attention_gradient_that_is_not_finite(dtype):
+  """An infinite or NaN gradient of one query spoils what it enters, never the gradients of masked tokens (zeros)."""
+  gen = torch.Generator().manual_seed(15)
+  q, k, v, dout = inputs(gen, dtype, 1, 40, 100, 2, 1, 32)
+  dout[0, 3, 0] = float('inf')
+  dout[0, 4, 1, 5] = float('nan')
+  mask = torch.rand(1, 100, generator=gen) < 0.5
+  with Ctx(dtype) as c:
+    out, dq, dk, dv = run_attention(c, q, k, v, None, mask, dout=dout)
+  assert (dk[~mask] == 0).all() and (dv[~mask] == 0).all() and torch.isfinite(out.float()).all()
+  fine = torch.ones(40, 2, dtype=torch.bool)
+  fine[3, 0] = fine[4, 1] = False
+  assert torch.isfinite(dq[0][fine].float()).all() and not torch.isfinite(dq[0][~fine].float()).all()
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
@@ -314,6 +363,7 @@ def test_refusals():
                   dict(scale=-1.0), dict(scale=float('nan')), dict(q=None), dict(k=p + 4), dict(v=None), dict(q_stride=10),
                   dict(k_stride=9), dict(v_stride=7)):
         assert attend(back, **bad) == INV, bad
+      assert attend(back, q_stride=1 << 22) == UNS and attend(back, k_stride=1 << 22) == UNS and attend(back, v_stride=-8) == UNS
       assert attend(back, queries=1 << 31) == UNS and attend(back, keys=1 << 31) == UNS and attend(back, batch=1 << 22) == UNS
     assert attend(out=None) == INV and attend(stats=None) == INV and attend(out_f32=None) == INV
     assert attend(True, stats=None) == INV and attend(True, out_f32=None) == INV and attend(True, dk=None) == INV

@@ -225,6 +225,56 @@ def test_cross_attention_strides(A, dtype):
   R.check('dv', dv, want[3])
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('batch,queries,keys', [(70, 3, 300), (70, 400, 200), (9, 70, 1500)])
+def test_cross_attention_many_clips(A, dtype, batch, queries, keys):
+  """More clips than a wave has lanes, of all lengths from none to whole."""
+  gen = generator(13)
+  inputs, dout = attention_inputs(gen, dtype, batch, queries, keys, 2, 1, 32)
+  lengths = torch.randint(0, keys + 1, (batch,), generator=gen, device='cuda').to(torch.int32)
+  lengths[0], lengths[1], lengths[-1], lengths[-2] = 0, keys, keys, 0
+  check_attention(A, inputs, dout, lengths)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_gradients_of_some_inputs(A, dtype):
+  """Only what is asked for is computed, with the bits of the whole backward pass; no second derivative."""
+  gen = generator(14)
+  inputs, dout = attention_inputs(gen, dtype, 2, 40, 300, 4, 2, 64)
+  lengths = torch.tensor([300, 11], dtype=torch.int32, device='cuda')
+  whole = grads_of(A.cross_attention(*inputs, key_lengths=lengths), inputs, dout)
+  for wanted in ([0], [1], [2], [0, 2], [1, 2]):
+    some = [t if n in wanted else t.detach() for n, t in enumerate(inputs)]
+    for args in (some, inputs):       # the others need no gradient, or none is asked for
+      got = grads_of(A.cross_attention(*args, key_lengths=lengths), [inputs[n] for n in wanted], dout)
+      assert all(torch.equal(g, whole[n]) for g, n in zip(got, wanted))
+  x = randn(gen, 5, 7, 32).to(dtype).requires_grad_()
+  weight, bias = randn(gen, 32).requires_grad_(), randn(gen, 32).requires_grad_()
+  all_of = grads_of(A.layer_norm(x, weight, bias).sum(), [x, weight, bias], None)
+  for n, t in enumerate((x, weight, bias)):
+    assert torch.equal(grads_of(A.layer_norm(x, weight, bias).sum(), [t], None)[0], all_of[n])
+  assert torch.equal(grads_of(A.layer_norm(x, None, bias).sum(), [bias], None)[0], all_of[2])
+  positions = torch.rand(40, 3, generator=gen, device='cuda')
+  for y, leaf in ((A.cross_attention(*inputs), inputs[0]), (A.layer_norm(x, weight, bias), x), (A.layer_norm(x), x),
+                  (A.rotary_positions(inputs[0], positions), inputs[0])):
+    (g,) = torch.autograd.grad(y.float().square().sum(), [leaf], create_graph=True, retain_graph=True)
+    with pytest.raises(RuntimeError, match='second derivative'):
+      g.sum().backward()
+    (g,) = torch.autograd.grad(y.float().square().sum(), [leaf], create_graph=True)
+    with pytest.raises(RuntimeError):
+      torch.autograd.grad(g.sum(), [leaf])
+
+
+def test_rows_far_apart(A):
+  """Tokens 2^22 elements and more apart: copied; a single token's stride does not matter."""
+  gen = generator(16)
+  (q, k, v), dout = attention_inputs(gen, torch.bfloat16, 1, 3, 5, 2, 2, 32, packed=False)
+  far = torch.zeros(5, 1 << 22, dtype=torch.bfloat16, device='cuda')[:, :64].view(1, 5, 2, 32)
+  far.copy_(k.detach())
+  assert far.stride(1) == 1 << 22
+  assert torch.equal(A.cross_attention(q, far, v), A.cross_attention(q, k, v))
+
+
 def test_cross_attention_gradient_against_differences(A):
   """Central differences of the float32 forward pass along random directions: the truncation is third order in the step, the
   outputs' own error (their bound) is divided by it."""
