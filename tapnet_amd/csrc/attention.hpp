@@ -147,7 +147,11 @@ __device__ __forceinline__ void at_operand2(const f32x16& p, unsigned (&w)[8], u
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const unsigned a = __float_as_uint(p[2 * i]) & 0xffff0000u, b = __float_as_uint(p[2 * i + 1]) & 0xffff0000u;
+#ifdef TAPIR_HIPEMU
     w[i] = (a >> 16) | b;
+#else
+    w[i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]), 0x07060302u);   // both upper halves
+#endif
     v[i] = pack_bf16x2(p[2 * i] - __uint_as_float(a), p[2 * i + 1] - __uint_as_float(b));
   }
 }
@@ -840,6 +844,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
       read(0);
 #pragma unroll
       for (int rb = 0; rb < RT; rb += 32) {
+        if (DP == 64 && rb > 0) read(rb);
         f32x16 s, g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -859,7 +864,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         }
 #pragma unroll
         for (int d = 0; d < NB; ++d) qx[d] = at_tr<CH>(qt[buf], rb, d * 32);
-        if (rb + 32 < RT) read(rb + 32);
+        if (DP != 64 && rb + 32 < RT) read(rb + 32);
         sched_fence();
         AtOperand<T> p, e, f;
 #pragma unroll
