@@ -85,7 +85,8 @@ void ln_bwd_dispatch(const LnBwdArgs& a, unsigned grid, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------------- attention
-int attn_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int attn_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+int attn_part(int dp) { return dp == 96 ? 128 : dp; }   // AtPart
 int attn_row_step(int dtype, int dp) { return dtype != TAPIR_BF16 && dp > 32 ? 32 : 64; }   // AtRowTile
 
 struct AttnPlan {
@@ -121,16 +122,17 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
   AttnPlan p{};
   const bool bf16 = dtype == TAPIR_BF16;
   p.dp = attn_pad(a->dim);
-  const int w = p.dp == 32 ? 0 : p.dp == 64 ? 1 : 2;
+  const int w = p.dp / 32 - 1;
   const long rows = (long)(a->heads / a->kv_heads) * a->queries, heads = std::max<long>(1, (long)a->batch * a->kv_heads);
   p.row_tiles = (int)((rows + AT_QROWS - 1) / AT_QROWS);
   const int kt = bf16 ? 64 : 32;
   const long tiles = std::max<long>(1, (a->keys + kt - 1) / kt);
   const double us_per_byte = 1 / 9e6;   // partial results, mostly out of the last-level cache
   // us a step of a workgroup that has its compute unit to itself, and workgroups a compute unit holds (AtWaves)
-  static const double fwd_us[2][3] = {{1.3, 2.6, 5.0}, {0.65, 0.92, 1.7}}, dq_us[2][3] = {{1.9, 3.6, 7.0}, {0.8, 1.2, 2.4}};
-  static const double dkv_us[2][3] = {{5.0, 5.0, 10.0}, {0.9, 1.4, 2.4}};
-  static const int fwd_occ[2][3] = {{4, 3, 1}, {4, 4, 2}}, dq_occ[2][3] = {{4, 2, 1}, {4, 3, 2}}, dkv_occ[2][3] = {{2, 2, 1}, {3, 2, 1}};
+  static const double fwd_us[2][4] = {{1.3, 2.6, 3.8, 5.0}, {0.65, 0.92, 1.3, 1.7}}, dq_us[2][4] = {{1.9, 3.6, 5.3, 7.0}, {0.8, 1.2, 1.8, 2.4}};
+  static const double dkv_us[2][4] = {{5.0, 5.0, 7.5, 10.0}, {0.9, 1.4, 1.9, 2.4}};
+  static const int fwd_occ[2][4] = {{4, 3, 2, 1}, {4, 4, 2, 2}}, dq_occ[2][4] = {{4, 2, 2, 1}, {4, 3, 2, 2}};
+  static const int dkv_occ[2][4] = {{2, 2, 1, 1}, {3, 2, 1, 1}};
   const double row_bytes = 8.0 * heads * rows * p.dp, key_bytes = 16.0 * heads * a->keys * p.dp;   // written and read
   // (a padded batch is taken to hold two thirds of its tokens: the lengths themselves are on the device)
   auto filled = [&](long units) { return std::max<long>(1, a->key_lengths ? units * 2 / 3 : units); };
@@ -140,7 +142,7 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
   if (!backward) {
     if (p.splits > 1) {
       const size_t r = (size_t)p.splits * a->batch * a->kv_heads * rows;
-      p.part_o = r * p.dp;
+      p.part_o = r * attn_part(p.dp);
       p.part_ml = round4(r * 2);
     }
     return p;
@@ -224,8 +226,8 @@ void attn_fwd_launch(const AttnArgs& k, hipStream_t s) {
   hipLaunchKernelGGL((attn_fwd_kernel<T, DP>), dim3(grid), dim3(AT_THREADS), 0, s, k);
   if (k.splits > 1) {
     const long rows = (long)k.B * k.Hkv * k.rows;
-    if (k.splits >= 32) hipLaunchKernelGGL((attn_join_kernel<T, DP, AT_WAVES>), dim3((unsigned)rows), dim3(AT_THREADS), 0, s, k);
-    else hipLaunchKernelGGL((attn_join_kernel<T, DP, 1>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k);
+    if (k.splits >= 32) hipLaunchKernelGGL((attn_join_kernel<T, AtPart<DP>::V, AT_WAVES>), dim3((unsigned)rows), dim3(AT_THREADS), 0, s, k);
+    else hipLaunchKernelGGL((attn_join_kernel<T, AtPart<DP>::V, 1>), dim3((unsigned)((rows + AT_WAVES - 1) / AT_WAVES)), dim3(AT_THREADS), 0, s, k);
   }
 }
 
@@ -246,13 +248,17 @@ void attn_bwd_launch(const AttnArgs& k, hipStream_t s) {
   if (join > 0) hipLaunchKernelGGL((attn_join_grads_kernel<T>), dim3(stride_grid((join / 4 + AT_THREADS - 1) / AT_THREADS)), dim3(AT_THREADS), 0, s, k);
 }
 
-#define ATTN_DISPATCH(fn, dtype, dp, ...)                                                                              \
-  do {                                                                                                                 \
-    if ((dtype) == TAPIR_BF16) {                                                                                       \
-      if ((dp) == 32) fn<bf16_t, 32>(__VA_ARGS__); else if ((dp) == 64) fn<bf16_t, 64>(__VA_ARGS__); else fn<bf16_t, 128>(__VA_ARGS__); \
-    } else {                                                                                                           \
-      if ((dp) == 32) fn<float, 32>(__VA_ARGS__); else if ((dp) == 64) fn<float, 64>(__VA_ARGS__); else fn<float, 128>(__VA_ARGS__);    \
-    }                                                                                                                  \
+#define ATTN_DISPATCH_T(fn, T, dp, ...)           \
+  do {                                            \
+    if ((dp) == 32) fn<T, 32>(__VA_ARGS__);       \
+    else if ((dp) == 64) fn<T, 64>(__VA_ARGS__);  \
+    else if ((dp) == 96) fn<T, 96>(__VA_ARGS__);  \
+    else fn<T, 128>(__VA_ARGS__);                 \
+  } while (0)
+#define ATTN_DISPATCH(fn, dtype, dp, ...)                                    \
+  do {                                                                       \
+    if ((dtype) == TAPIR_BF16) ATTN_DISPATCH_T(fn, bf16_t, dp, __VA_ARGS__); \
+    else ATTN_DISPATCH_T(fn, float, dp, __VA_ARGS__);                        \
   } while (0)
 
 }  // namespace

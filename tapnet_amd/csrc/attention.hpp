@@ -63,6 +63,10 @@ template <int CH> __device__ __forceinline__ int at_swizzle(int r, int c) {
 template <typename T> struct AtFrag;            // 16 bytes of a row: the operand of one k-step
 template <> struct AtFrag<bf16_t> { static constexpr int EPC = 8; };
 template <> struct AtFrag<float> { static constexpr int EPC = 4; };
+// chunks from row to row of a tile of DP channels: the swizzle stays within a power of two or a multiple of eight
+template <typename T, int DP> struct AtPitch { static constexpr int CH = DP / AtFrag<T>::EPC, V = CH % 8 == 0 || CH == 4 ? CH : 16; };
+// channels from row to row of the forward pass' partial results
+template <int DP> struct AtPart { static constexpr int V = DP == 96 ? 128 : DP; };
 
 // c += a b over the elements of one 16-byte chunk per lane (lanes l and l ^ 32 hold neighbouring chunks)
 __device__ __forceinline__ f32x16 at_mma(const uint4& a, const uint4& b, f32x16 c, bf16_t) {
@@ -205,7 +209,7 @@ __device__ __forceinline__ void at_copy16(const void* base, unsigned off, void* 
 // ROWS x DP tile of a [token][channel] tensor -> LDS, 16-byte chunks, by the whole workgroup: thread i copies slots i, i + 256,
 // ... of the tile.  The offsets of a thread's chunks from the tile's first row stay the same for all tiles of a tensor.
 template <typename T, int ROWS, int DP> struct AtStage {
-  static constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, N = ROWS * CH / AT_THREADS;
+  static constexpr int EPC = AtFrag<T>::EPC, CH = AtPitch<T, DP>::V, N = ROWS * CH / AT_THREADS;
   static_assert(ROWS * CH % AT_THREADS == 0, "tile");
   unsigned off[N];     // bytes (token strides are below AT_MAX_STRIDE elements)
 
@@ -390,8 +394,8 @@ __device__ __forceinline__ bool at_key_unit(const AttnArgs& a, AtUnit* u, bool* 
 // waves per SIMD that the register allocation aims at
 template <typename T, int DP> struct AtWaves {
   static constexpr bool BF16 = sizeof(T) == 2;
-  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? (BF16 ? 4 : 3) : (BF16 ? 2 : 1);
-  static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : (BF16 ? 2 : 1);
+  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? (BF16 ? 4 : 3) : DP == 96 ? 2 : (BF16 ? 2 : 1);
+  static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : DP == 96 ? 2 : (BF16 ? 2 : 1);
   static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
 };
 
@@ -400,9 +404,9 @@ template <typename T, int DP> struct AtWaves {
 // flight under the current tile's products.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_kernel(AttnArgs a) {
-  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
-  __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
-  __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
+  __shared__ __attribute__((aligned(16))) T kt[2][KT * PC * EPC];
+  __shared__ __attribute__((aligned(16))) T vt[2][KT * PC * EPC];
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
   AtUnit unit;
   if (!at_row_unit<T>(a, &unit)) return;
@@ -459,7 +463,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
     for (int kb = 0; kb < KT / 32; ++kb) {
       s[kb] = at_zero();
 #pragma unroll
-      for (int x = 0; x < CH / 2; ++x) s[kb] = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s[kb], T{});
+      for (int x = 0; x < CH / 2; ++x) s[kb] = at_mma(at_chunk<T, PC>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s[kb], T{});
       const unsigned mb = (unsigned)(cur >> (32 * kb));
       if (mb != 0xffffffffu) {
         const unsigned mine = mb >> (4 * h);
@@ -491,14 +495,14 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
       at_operand(s[kb], p.w);
       sum = at_sum(s[kb], sum);
 #pragma unroll
-      for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], vt[buf], kb * 32, d * 32, p.w);
+      for (int d = 0; d < NB; ++d) at_mma_tr<PC>(o[d], vt[buf], kb * 32, d * 32, p.w);
     }
   }
   sum = at_sum_halves(sum);
   if (!live) return;
   const long bh = (long)b * a.Hkv + hk;
   if (a.splits > 1) {
-    float* po = a.part_o + (((long)split * a.B * a.Hkv + bh) * a.rows + row) * DP;
+    float* po = a.part_o + (((long)split * a.B * a.Hkv + bh) * a.rows + row) * AtPart<DP>::V;
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -584,10 +588,10 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
 // joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
-  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, KT = AtTile<T>::KT, NB = DP / 32;
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
   constexpr bool BF16 = sizeof(T) == 2;
-  __shared__ __attribute__((aligned(16))) T kt[2][KT * DP];
-  __shared__ __attribute__((aligned(16))) T vt[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) T kt[2][KT * PC * EPC];
+  __shared__ __attribute__((aligned(16))) T vt[2][KT * PC * EPC];
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
   AtUnit unit;
   if (!at_row_unit<T>(a, &unit)) return;
@@ -660,8 +664,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
       f32x16 s = at_zero(), g = BF16 ? minus_delta : at_zero();
 #pragma unroll
       for (int x = 0; x < CH / 2; ++x) {
-        s = at_mma(at_chunk<T, CH>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
-        g = at_mma(at_chunk<T, CH>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
+        s = at_mma(at_chunk<T, PC>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
+        g = at_mma(at_chunk<T, PC>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (BF16 ? g[i] : g[i] - delta);
@@ -676,7 +680,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
         at_operand2(s, w, v);
 #pragma unroll
         for (int d = 0; d < NB; ++d) {
-          const AtTr x = at_tr<CH>(kt[buf], kb * 32, d * 32);
+          const AtTr x = at_tr<PC>(kt[buf], kb * 32, d * 32);
           at_mma_tr(o[d], x, w);
           at_mma_tr(o[d], x, v);
         }
@@ -684,7 +688,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
         AtOperand<T> p;
         at_operand(s, p.w);
 #pragma unroll
-        for (int d = 0; d < NB; ++d) at_mma_tr<CH>(o[d], kt[buf], kb * 32, d * 32, p.w);
+        for (int d = 0; d < NB; ++d) at_mma_tr<PC>(o[d], kt[buf], kb * 32, d * 32, p.w);
       }
     }
   }
@@ -724,9 +728,9 @@ __global__ __launch_bounds__(AT_THREADS) void attn_delta_kernel(AttnArgs a) {
 // dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads (or a split of them), RT at a time.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_kernel(AttnArgs a) {
-  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
-  __shared__ __attribute__((aligned(16))) T qt[2][RT * DP];
-  __shared__ __attribute__((aligned(16))) T gt[2][RT * DP];
+  constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
+  __shared__ __attribute__((aligned(16))) T qt[2][RT * PC * EPC];
+  __shared__ __attribute__((aligned(16))) T gt[2][RT * PC * EPC];
   // what the rows' products start from and are multiplied by.  bf16: the products begin at -log2(e) L_r / scale2 and -D_r (L_r =
   // m_r + log l_r), so that p = exp2(scale2 s) and ds = p dp remain; f32: m_r, D_r and 1 / l_r apart, because one number L_r would
   // be rounded at its own size (2^-21 at 10, a relative error of 5 u of the whole row).
@@ -837,14 +841,14 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
       auto read = [&](int rb) {
 #pragma unroll
         for (int x = 0; x < CH / 2; ++x) {
-          qa[x] = at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h);
-          ga[x] = at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h);
+          qa[x] = at_chunk<T, PC>(qt[buf], rb + (l & 31), 2 * x + h);
+          ga[x] = at_chunk<T, PC>(gt[buf], rb + (l & 31), 2 * x + h);
         }
       };
       read(0);
 #pragma unroll
       for (int rb = 0; rb < RT; rb += 32) {
-        if (DP == 64 && rb > 0) read(rb);
+        if ((DP == 64 || DP == 96) && rb > 0) read(rb);
         f32x16 s, g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -855,7 +859,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         }
         AtTr gx[NB], qx[NB];
 #pragma unroll
-        for (int d = 0; d < NB; ++d) gx[d] = at_tr<CH>(gt[buf], rb, d * 32);
+        for (int d = 0; d < NB; ++d) gx[d] = at_tr<PC>(gt[buf], rb, d * 32);
         sched_fence();
 #pragma unroll
         for (int x = 0; x < CH / 2; ++x) {
@@ -863,8 +867,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
           g = at_mma(ga[x], vf[x], g, T{});
         }
 #pragma unroll
-        for (int d = 0; d < NB; ++d) qx[d] = at_tr<CH>(qt[buf], rb, d * 32);
-        if (DP != 64 && rb + 32 < RT) read(rb + 32);
+        for (int d = 0; d < NB; ++d) qx[d] = at_tr<PC>(qt[buf], rb, d * 32);
+        if ((DP == 32 || DP == 128) && rb + 32 < RT) read(rb + 32);
         sched_fence();
         AtOperand<T> p, e, f;
 #pragma unroll
@@ -888,8 +892,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         f32x16 s = at_zero(), g = at_zero();
 #pragma unroll
         for (int x = 0; x < CH / 2; ++x) {
-          s = at_mma(at_chunk<T, CH>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
-          g = at_mma(at_chunk<T, CH>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
+          s = at_mma(at_chunk<T, PC>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
+          g = at_mma(at_chunk<T, PC>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -907,8 +911,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         at_operand(g, e.w);
 #pragma unroll
         for (int d = 0; d < NB; ++d) {
-          at_mma_tr<CH>(dv[d], gt[buf], rb, d * 32, p.w);
-          at_mma_tr<CH>(dk[d], qt[buf], rb, d * 32, e.w);
+          at_mma_tr<PC>(dv[d], gt[buf], rb, d * 32, p.w);
+          at_mma_tr<PC>(dk[d], qt[buf], rb, d * 32, e.w);
         }
       }
     }
