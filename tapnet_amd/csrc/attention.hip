@@ -131,7 +131,7 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
   // us a step of a workgroup that has its compute unit to itself, and workgroups a compute unit holds (AtWaves)
   static const double fwd_us[2][4] = {{1.3, 2.6, 3.8, 5.0}, {0.65, 0.92, 1.3, 1.7}}, dq_us[2][4] = {{1.9, 3.6, 5.3, 7.0}, {0.8, 1.2, 1.8, 2.4}};
   static const double dkv_us[2][4] = {{5.0, 5.0, 7.5, 10.0}, {0.9, 1.4, 1.9, 2.4}};
-  static const int fwd_occ[2][4] = {{4, 3, 2, 1}, {4, 4, 2, 2}}, dq_occ[2][4] = {{4, 2, 2, 1}, {4, 3, 2, 2}};
+  static const int fwd_occ[2][4] = {{4, 3, 2, 1}, {4, 4, 2, 2}}, dq_occ[2][4] = {{4, 2, 1, 1}, {4, 3, 2, 2}};
   static const int dkv_occ[2][4] = {{2, 2, 1, 1}, {3, 2, 1, 1}};
   const double row_bytes = 8.0 * heads * rows * p.dp, key_bytes = 16.0 * heads * a->keys * p.dp;   // written and read
   // (a padded batch is taken to hold two thirds of its tokens: the lengths themselves are on the device)

@@ -126,12 +126,15 @@ __device__ __forceinline__ void at_mma_tr(f32x16& c, const bf16_t* X, int r0, in
 template <int CH>
 __device__ __forceinline__ void at_mma_tr(f32x16& c, const float* X, int r0, int d0, const float (&w)[16]) {
   const int l = threadIdx.x & 63, h = l >> 5, col = d0 + (l & 31);
+  float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = r0 + 8 * (i >> 2) + 4 * h + (i & 3);
-    const float x = X[((long)r * CH + at_swizzle<CH>(r, col >> 2)) * 4 + (col & 3)];
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x, w[i], c, 0, 0, 0);
+    x[i] = X[((long)r * CH + at_swizzle<CH>(r, col >> 2)) * 4 + (col & 3)];
   }
+  sched_fence();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], w[i], c, 0, 0, 0);
 }
 
 // the 16 values of a lane as the operand of at_mma_tr: as they are (f32), or rounded to bf16.  The forward pass rounds p once: its
@@ -240,6 +243,22 @@ template <typename T, int ROWS, int DP> struct AtStage {
 
 template <typename T, int CH> __device__ __forceinline__ uint4 at_chunk(const T* X, int r, int c) {
   return *reinterpret_cast<const uint4*>(X + ((long)r * CH + at_swizzle<CH>(r, c)) * AtFrag<T>::EPC);
+}
+
+// s += (rows r + lane of the tile X) . (the lane's operand chunks b), f32: the next chunk is read before the products with this one
+// are issued, and a fence keeps it so (the compiler would read each right before its products and wait; 739 x 1161 x 32 x 72,
+// backward: 527 -> 472 us.  bf16, whose products take an eighth of the time, gains nothing by one chunk and spills with more)
+template <typename T, int PC, int NS>
+__device__ __forceinline__ void at_dot(f32x16& s, const T* X, int r, const uint4 (&b)[NS]) {
+  const int l = threadIdx.x & 63, h = l >> 5;
+  uint4 a[2];
+  a[0] = at_chunk<T, PC>(X, r + (l & 31), h);
+#pragma unroll
+  for (int x = 0; x < NS; ++x) {
+    if (x + 1 < NS) a[(x + 1) & 1] = at_chunk<T, PC>(X, r + (l & 31), 2 * x + 2 + h);
+    sched_fence();
+    s = at_mma(a[x & 1], b[x], s, T{});
+  }
 }
 
 // Key validity of a tile's keys as a wave-uniform mask (bit j: key k0 + j takes part).  The mask's bytes are read one tile ahead:
@@ -395,7 +414,7 @@ __device__ __forceinline__ bool at_key_unit(const AttnArgs& a, AtUnit* u, bool* 
 template <typename T, int DP> struct AtWaves {
   static constexpr bool BF16 = sizeof(T) == 2;
   static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? (BF16 ? 4 : 3) : DP == 96 ? 2 : (BF16 ? 2 : 1);
-  static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : DP == 96 ? 2 : (BF16 ? 2 : 1);
+  static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : BF16 ? 2 : 1;
   static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
 };
 
@@ -662,10 +681,15 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       f32x16 s = at_zero(), g = BF16 ? minus_delta : at_zero();
+      if constexpr (sizeof(T) == 4 && DP > 64) {
+        at_dot<T, PC>(s, kt[buf], kb * 32, qf);
+        at_dot<T, PC>(g, vt[buf], kb * 32, gf);
+      } else {
 #pragma unroll
-      for (int x = 0; x < CH / 2; ++x) {
-        s = at_mma(at_chunk<T, PC>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
-        g = at_mma(at_chunk<T, PC>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
+        for (int x = 0; x < CH / 2; ++x) {
+          s = at_mma(at_chunk<T, PC>(kt[buf], kb * 32 + (l & 31), 2 * x + h), qf[x], s, T{});
+          g = at_mma(at_chunk<T, PC>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (BF16 ? g[i] : g[i] - delta);
@@ -890,11 +914,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
 #pragma unroll
       for (int rb = 0; rb < RT; rb += 32) {
         f32x16 s = at_zero(), g = at_zero();
-#pragma unroll
-        for (int x = 0; x < CH / 2; ++x) {
-          s = at_mma(at_chunk<T, PC>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
-          g = at_mma(at_chunk<T, PC>(gt[buf], rb + (l & 31), 2 * x + h), vf[x], g, T{});
-        }
+        at_dot<T, PC>(s, qt[buf], rb, kf);
+        at_dot<T, PC>(g, gt[buf], rb, vf);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const tapir_f32x4 M = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
