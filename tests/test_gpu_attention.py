@@ -169,7 +169,7 @@ def check_attention(A, inputs, dout, lengths=None, mask=None, scale=None):
 @pytest.mark.parametrize('batch,queries,keys,heads,kv_heads,dim', [
     (1, 1, 1, 1, 1, 8), (1, 1, 4099, 8, 2, 64), (2, 3, 33, 4, 4, 32), (1, 257, 1024, 8, 8, 32), (1, 31, 3000, 4, 1, 128),
     (3, 129, 65, 6, 2, 96), (1, 2, 20000, 4, 4, 64), (1, 2000, 17, 4, 2, 40), (1, 700, 1900, 2, 2, 64), (2, 5, 0, 2, 2, 32),
-    (2, 0, 7, 2, 1, 32), (1, 64, 64, 1, 1, 120)])
+    (2, 0, 7, 2, 1, 32), (1, 64, 64, 1, 1, 120), (2, 200, 700, 4, 2, 72), (1, 65, 130, 2, 1, 88), (1, 9, 3000, 8, 2, 96), (2, 520, 40, 4, 1, 104)])
 def test_cross_attention(A, dtype, batch, queries, keys, heads, kv_heads, dim):
   gen = generator(queries * 7 + keys)
   inputs, dout = attention_inputs(gen, dtype, batch, queries, keys, heads, kv_heads, dim)
