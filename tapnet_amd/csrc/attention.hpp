@@ -231,7 +231,7 @@ template <typename T, int ROWS, int DP> struct AtStage {
   // rows from `first` on; row r is zeros where bit r of `bits` is not set, channels from D on are zeros too
   __device__ __forceinline__ void rows(T* lds, const T* first, uint64_t bits, int D) const {
     constexpr uint64_t all = ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
-    if ((bits & all) == all && D == DP) {
+    if ((bits & all) == all && D == CH * EPC) {   // (no chunk of the pitch lies behind the channels)
 #pragma unroll
       for (int n = 0; n < N; ++n) at_copy16(first, off[n], lds + (n * AT_THREADS + (threadIdx.x >> 6) * 64) * EPC);
     } else {

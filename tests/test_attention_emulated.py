@@ -1,6 +1,10 @@
 """Layer normalisation, rotary positions and cross attention (csrc/layer_norm.hpp, rotary.hpp, attention.hpp) through the C ABI
 on the host emulator, against 64-bit forms with counted roundings (tests/attention_ref.py); the entry points' refusals."""
 import ctypes
+import mmap
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -305,6 +309,49 @@ def test_cross_attention_large_scores(dtype):
     got = run_attention(c, q, k, v, scale=2.0, dout=dout)
   for name, g, w in zip(('out', 'dq', 'dk', 'dv'), got, R.attention(q, k, v, torch.ones(1, keys, dtype=torch.bool), 2.0, dout)):
     R.check(name, g, w)
+
+
+# ------------------------------------------------------------------------------------------------ reads stay inside
+def before_a_guard_page(t):
+  """A copy of the tensor whose last byte is followed by a page that may not be touched."""
+  nbytes = t.numel() * t.element_size()
+  pages = -(-nbytes // mmap.PAGESIZE)
+  region = mmap.mmap(-1, (pages + 1) * mmap.PAGESIZE)
+  start = ctypes.addressof(ctypes.c_char.from_buffer(region))
+  libc = ctypes.CDLL(None, use_errno=True)
+  assert libc.mprotect(ctypes.c_void_p(start + pages * mmap.PAGESIZE), ctypes.c_size_t(mmap.PAGESIZE), 0) == 0
+  at = np.frombuffer(region, dtype=np.uint8, count=nbytes, offset=pages * mmap.PAGESIZE - nbytes)
+  out = torch.from_numpy(at).view(t.dtype).view(t.shape)
+  out.copy_(t)
+  return out
+
+
+def reads_up_to_the_last_byte():
+  gen = torch.Generator().manual_seed(17)
+  for dtype in DTYPES:
+    for queries, keys, dim in ((64, 64, 96), (128, 192, 96), (70, 130, 72), (3, 64, 128), (33, 70, 40), (64, 64, 64), (1, 1, 8), (130, 257, 104)):
+      q, k, v, dout = (before_a_guard_page(t.contiguous()) for t in inputs(gen, dtype, 1, queries, keys, 2, 1, dim))
+      mask = before_a_guard_page(torch.ones(1, keys, dtype=torch.bool))
+      lengths = before_a_guard_page(torch.tensor([keys, ], dtype=torch.int32))
+      print(dtype, queries, keys, dim, flush=True)
+      with Ctx(dtype) as c:
+        run_attention(c, q, k, v, dout=dout)
+        run_attention(c, q, k, v, lengths, mask, dout=dout)
+        x = before_a_guard_page(torch.randn(1, 5, 2, dim, generator=gen).to(dtype))
+        run_rotary(c, x, before_a_guard_page(torch.rand(1, 5, 1, generator=gen)), [dim // 2 // 2 * 2], [100.0], False)
+        rows = before_a_guard_page(torch.randn(9, dim + 1, generator=gen).to(dtype))
+        run_layer_norm(c, rows, before_a_guard_page(torch.rand(dim + 1, generator=gen)), None, 1e-5, rows)
+        rows = before_a_guard_page(torch.randn(9, dim, generator=gen).to(dtype))
+        run_layer_norm(c, rows, before_a_guard_page(torch.rand(dim, generator=gen)), None, 1e-5, rows)
+
+
+def test_reads_stay_inside():
+  """Inputs that end where memory ends, in a process of its own (a read behind them ends it)."""
+  root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+  emu_lib()
+  done = subprocess.run([sys.executable, '-c', 'from tests import test_attention_emulated as t; t.reads_up_to_the_last_byte(); print("all")'],
+                        cwd=root, capture_output=True, text=True, timeout=600)
+  assert done.returncode == 0 and done.stdout.endswith('all\n'), (done.returncode, done.stdout[-300:], done.stderr[-600:])
 
 
 # ----------------------------------------------------------------------------------------------------- refusals
