@@ -1,0 +1,73 @@
+"""Cross attention on the host emulator against tests/attention_tight.py: long sums, tokens that each show in a result, and what the
+bounds reject (mistakes planted in the oracle)."""
+import pytest
+import torch
+
+from tests import attention_tight as N
+from tests import test_attention_emulated as E
+
+DTYPES, IDS = E.DTYPES[:1], E.IDS[:1]
+
+
+def all_of(k):
+  return torch.ones(k.shape[:2], dtype=torch.bool)
+
+
+def compare(c, q, k, v, dout, keep=None, **how):
+  got = E.run_attention(c, q, k, v, dout=dout, **how)
+  want = N.attention(q, k, v, all_of(k) if keep is None else keep, q.shape[-1] ** -0.5, dout)
+  for name, g, w in zip(('out', 'dq', 'dk', 'dv'), got, want[1:]):
+    N.check(name, g, w)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('keys,heads,kv_heads,dim', [(65, 1, 1, 32), (700, 2, 1, 64), (2111, 1, 1, 40), (1025, 1, 1, 128), (640, 1, 1, 96)])
+def test_every_token_counts(dtype, keys, heads, kv_heads, dim):
+  gen = torch.Generator().manual_seed(keys)
+  q, k, v, dout, at = N.dominated(gen, dtype, 'cpu', keys, heads, kv_heads, dim, most=40)
+  with E.Ctx(dtype) as c:
+    compare(c, q, k, v, dout)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('queries,keys,dim', [(1, 4099, 64), (3, 2000, 32), (130, 600, 24)])
+def test_rows_that_attend_to_everything(dtype, queries, keys, dim):
+  """Probabilities of like size: the results are small sums of many terms, in which every rounding of p shows."""
+  gen = torch.Generator().manual_seed(keys + 1)
+  q, k, v, dout = E.inputs(gen, dtype, 1, queries, keys, 2, 1, dim)
+  q = (0.3 * torch.randn(q.shape, generator=gen)).to(dtype)
+  with E.Ctx(dtype) as c:
+    compare(c, q, k, v, dout)
+
+
+@pytest.mark.parametrize('dtype', E.DTYPES, ids=E.IDS)
+def test_the_bounds_reject_mistakes(dtype):
+  """Oracles that leave out the last 8 of 4099 keys, count one key twice, or round p and ds once to bf16 are outside the bounds."""
+  keys, dim = 4099, 64
+  gen = torch.Generator().manual_seed(5)
+  q = (0.3 * torch.randn(1, 4, 1, dim, generator=gen)).to(dtype)
+  k, v = (torch.randn(1, keys, 1, dim, generator=gen).to(dtype) for _ in range(2))
+  dout = torch.randn(1, 4, 1, dim, generator=gen).to(dtype)
+  want = N.attention(q, k, v, all_of(k), dim ** -0.5, dout)
+  short = all_of(k)
+  short[:, -8:] = False
+
+  def rejected(values):
+    out = []
+    for (value, bound), other in zip(want[1:], values):
+      out.append(bool(((other.to(dtype).double() - value).abs() > bound).any()))
+    return out
+  assert all(rejected([w[0] for w in N.attention(q, k, v, short, dim ** -0.5, dout)[1:]]))
+  assert not any(rejected([w[0] for w in want[1:]]))
+  twice = torch.cat([torch.arange(keys), torch.tensor([keys - 1])])
+  kk, vv = k[:, twice], v[:, twice]
+  other = [w[0] for w in N.attention(q, kk, vv, all_of(kk), dim ** -0.5, dout)[1:]]
+  other[2:] = [torch.cat([t[:, :keys - 1], t[:, keys - 1:].sum(1, keepdim=True)], 1) for t in other[2:]]
+  assert any(rejected(other))
+  if dtype == torch.bfloat16:
+    once = lambda t: t.to(torch.bfloat16).double()
+    Q, K, V, D = (t.double()[0, :, 0] for t in (q, k, v, dout))
+    p = torch.softmax(Q @ K.T * dim ** -0.5, -1)
+    ds = p * (D @ V.T - (D * (p @ V)).sum(-1, keepdim=True)) * dim ** -0.5
+    shape = lambda t: t[None, :, None]
+    assert all(rejected([shape(once(p) @ V), shape(once(ds) @ K), shape(once(ds).T @ Q), shape(once(p).T @ D)]))

@@ -1,0 +1,57 @@
+"""Cross attention on an MI355X against tests/attention_tight.py: over many keys, with tokens at the ends of tiles and splits that each
+show in a result."""
+import pytest
+import torch
+
+from tests import attention_tight as N
+from tests import test_gpu_attention as T
+
+pytestmark = pytest.mark.gpu
+
+DTYPES, IDS = T.DTYPES[:1], T.IDS[:1]
+A = T.A
+
+
+def compare(A, q, k, v, dout, lengths=None, mask=None):
+  inputs = [t.detach().requires_grad_() for t in (q, k, v)]
+  keep = torch.ones(k.shape[:2], dtype=torch.bool, device='cuda') if mask is None else mask.clone()
+  if lengths is not None:
+    keep &= torch.arange(k.shape[1], device='cuda') < lengths[:, None].long()
+  out = A.cross_attention(*inputs, key_lengths=lengths, key_mask=mask)
+  grads = T.grads_of(out, inputs, dout)
+  with torch.no_grad():
+    want = N.attention(q, k, v, keep, q.shape[-1] ** -0.5, dout)
+    for name, g, w in zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *grads), want[1:]):
+      N.check(name, g, w)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('keys,heads,kv_heads,dim,most', [
+    (4099, 2, 1, 64, 96), (20000, 4, 4, 64, 8), (20000, 2, 2, 32, 400), (49152, 1, 1, 64, 32), (8200, 4, 2, 128, 300), (3001, 2, 1, 96, 64),
+    (129, 1, 1, 8, 64)])
+def test_every_token_counts(A, dtype, keys, heads, kv_heads, dim, most):
+  gen = T.generator(keys + dim)
+  q, k, v, dout, _ = N.dominated(gen, dtype, 'cuda', keys, heads, kv_heads, dim, most)
+  compare(A, q, k, v, dout)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_the_last_token_of_every_clip_counts(A, dtype):
+  """A padded batch whose lengths end inside a tile, behind one and before one."""
+  gen = T.generator(50)
+  q, k, v, dout, _ = N.dominated(gen, dtype, 'cuda', 5000, 2, 1, 64, 8)
+  lengths = torch.tensor([5000, 4097, 4096, 4095, 1, 65, 640, 2048], dtype=torch.int32, device='cuda')
+  k, v = (t.expand(len(lengths), -1, -1, -1).contiguous() for t in (k, v))
+  ends = k[torch.arange(len(lengths)), (lengths.long() - 1).tolist()][:, None].float().repeat_interleave(2, 2)
+  q = (ends * (T.math.log(5000) + 2.2) * 8).to(dtype).expand(-1, 3, -1, -1).contiguous()
+  compare(A, q, k, v, T.randn(gen, len(lengths), 3, 2, 64).to(dtype), lengths)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('queries,keys,heads,kv_heads,dim', [
+    (1, 49152, 8, 2, 64), (3, 20000, 4, 4, 32), (256, 1024, 8, 8, 32), (1000, 4099, 2, 1, 64), (300, 3000, 2, 2, 128), (5, 4099, 2, 1, 104)])
+def test_rows_that_attend_to_everything(A, dtype, queries, keys, heads, kv_heads, dim):
+  """Probabilities of like size: the results are small sums of many terms, in which every rounding of p shows."""
+  gen = T.generator(keys + queries)
+  (_, k, v), dout = T.attention_inputs(gen, dtype, 1, queries, keys, heads, kv_heads, dim)
+  compare(A, (0.3 * T.randn(gen, 1, queries, heads, dim)).to(dtype), k.detach(), v.detach(), dout)
