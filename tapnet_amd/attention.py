@@ -79,6 +79,6 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
   ``dim ** -0.5``.
 
   Returns ``[batch, queries, heads, dim]`` in q's type.  Scores, statistics and sums are float32; in bfloat16 the
-  forward pass rounds the probabilities to bfloat16 on their way into the second product (the gradients keep 16 bits of them).
+  probabilities and the scores' gradients enter the second products with 16 bits, twice bfloat16's eight.
   In float32 the result itself is kept for the backward pass, as softmax keeps its own: overwriting it in place is an error there."""
   return _ops().cross_attention(q, k, v, key_lengths, key_mask, scale)

@@ -98,7 +98,7 @@ size_t round4(size_t n) { return (n + 3) & ~(size_t)3; }   // (shares of a works
 
 // Splits of a long axis: `base` workgroups of `steps` steps each become base * s of steps / s, joined at `join` us a split.  The s of
 // the least estimated time is taken.  Estimate: n workgroups that share a compute unit (of 256) take t1 max(1 + (n - 1) / 2, 0.7 n)
-// a step (4096 queries x 49152 keys x 64, forward: 0.92, 1.37, 1.93, 2.55 us for 1 to 4), `occupancy` of them at once, and three
+// a step (24576 keys x 64, forward: 1.11, 1.74, 2.49 us for 1 to 3), `occupancy` of them at once, and three
 // steps' time to begin.  Measured, 256 x 49152 x 4 x 64: forward 699 us unsplit, 34 / 30 / 32 / 34 / 39 us for 256 / 512 / 768 / 1024 /
 // 1536 workgroups; 3 x 1000 x 8200 x 2 x 128: backward 169 us with the rows of dk / dv unsplit, 189 / 202 / 224 us with 2 / 3 / 6 splits.
 struct AttnSplit { long steps, base; int occupancy; double t1, join, join_first; };
@@ -129,9 +129,9 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
   const long tiles = std::max<long>(1, (a->keys + kt - 1) / kt);
   const double us_per_byte = 1 / 9e6;   // partial results, mostly out of the last-level cache
   // us a step of a workgroup that has its compute unit to itself, and workgroups a compute unit holds (AtWaves)
-  static const double fwd_us[2][4] = {{1.3, 2.6, 3.8, 5.0}, {0.65, 0.92, 1.3, 1.7}}, dq_us[2][4] = {{1.9, 3.6, 5.3, 7.0}, {0.8, 1.2, 1.8, 2.4}};
+  static const double fwd_us[2][4] = {{1.3, 2.6, 3.8, 5.0}, {0.9, 1.1, 1.7, 1.6}}, dq_us[2][4] = {{1.9, 3.6, 5.3, 7.0}, {0.8, 1.2, 1.8, 2.4}};
   static const double dkv_us[2][4] = {{5.0, 5.0, 7.5, 10.0}, {0.9, 1.4, 1.9, 2.4}};
-  static const int fwd_occ[2][4] = {{4, 3, 2, 1}, {4, 4, 2, 2}}, dq_occ[2][4] = {{4, 2, 1, 1}, {4, 3, 2, 2}};
+  static const int fwd_occ[2][4] = {{4, 3, 2, 1}, {4, 3, 2, 2}}, dq_occ[2][4] = {{4, 2, 1, 1}, {4, 3, 2, 2}};
   static const int dkv_occ[2][4] = {{2, 2, 1, 1}, {3, 2, 1, 1}};
   const double row_bytes = 8.0 * heads * rows * p.dp, key_bytes = 16.0 * heads * a->keys * p.dp;   // written and read
   // (a padded batch is taken to hold two thirds of its tokens: the lengths themselves are on the device)

@@ -137,19 +137,16 @@ __device__ __forceinline__ void at_mma_tr(f32x16& c, const float* X, int r0, int
   for (int i = 0; i < 16; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], w[i], c, 0, 0, 0);
 }
 
-// the 16 values of a lane as the operand of at_mma_tr: as they are (f32), or rounded to bf16.  The forward pass rounds p once: its
-// weights of one sign add up, the error (2^-8 a term at most, a third of that on average) stays near the output's own rounding.
-__device__ __forceinline__ void at_operand(const f32x16& p, unsigned (&w)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-}
+// the 16 values of a lane as the operand of at_mma_tr, f32: as they are
 __device__ __forceinline__ void at_operand(const f32x16& p, float (&w)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = p[i];
 }
-// The same in two parts, w + v: the 16 most significant bits and the bf16 of what is left (2^-16 together).  The gradients take this
-// way: their terms have either sign and cancel in part, and with one rounding of ds and p the gradients were 1.45 to 1.7 times as far
-// from the exact ones as their own final rounding is (256 queries x 49152 keys: 6 us of 95 for p, 10 us for ds).
+// bf16: in two parts, w + v: the 16 most significant bits and the bf16 of what is left (2^-15 together).  One rounding of p and ds
+// would show: where a row attends to many tokens alike its result is a small sum of many terms, and the error of p stands beside the
+// result's own rounding (1.4 to 1.5 times as far from the exact result in all; 1 query x 49152 keys); the gradients' terms cancel as well
+// (1.45 to 1.7 times).  What the second part costs, forward: 1 query x 49152 keys, 8 / 2 heads x 64: 14.7 -> 15.3 us; 256 x 49152 x 4 x 64:
+// 30.6 -> 34.5; 4096 x 49152 x 4 x 64: 260 -> 337 (the vector unit splits every p); gradients, 256 x 49152: 6 us of 95 for p, 10 for ds.
 __device__ __forceinline__ void at_operand2(const f32x16& p, unsigned (&w)[8], unsigned (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -413,16 +410,17 @@ __device__ __forceinline__ bool at_key_unit(const AttnArgs& a, AtUnit* u, bool* 
 // waves per SIMD that the register allocation aims at
 template <typename T, int DP> struct AtWaves {
   static constexpr bool BF16 = sizeof(T) == 2;
-  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? (BF16 ? 4 : 3) : DP == 96 ? 2 : (BF16 ? 2 : 1);
+  static constexpr int FWD = DP == 32 ? 4 : DP == 64 ? 3 : DP == 96 ? 2 : (BF16 ? 2 : 1);
   static constexpr int DQ = DP == 32 ? 4 : DP == 64 ? (BF16 ? 3 : 2) : BF16 ? 2 : 1;
   static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
 };
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // A workgroup: AT_QROWS query rows of one key head, `tiles_per_split` key tiles; two LDS buffers, the next tile's copies in
-// flight under the current tile's products.  A score costs a multiply-add, an exponential (two issue slots), half a maximum, an addition and
-// half a conversion: bound by the vector unit (two thirds busy) next to a third of the matrix unit's time; four waves a SIMD overlap the two (three: 277 us).  4096 x 49152 x 4 x 64, bf16: 251-265 us, 0.8 PFLOP/s; 256 x 49152:
-// 25 us, 0.5 PFLOP/s; f32 256 x 4096 x 16 x 32: 28 us, 77 TFLOP/s of 151.
+// flight under the current tile's products.  A score costs the vector unit a multiply-add, an exponential (two issue slots), half a
+// maximum, an addition and three operations that split it in two parts (and, subtract, half a conversion, half a permutation): bound by
+// that next to three products.  Three waves a SIMD at 64 channels hold the operands (161 registers; at four they spill: 373 us
+// for 337).  4096 x 49152 x 4 x 64, bf16: 337 us with the join, 0.92 PFLOP/s executed; f32 256 x 4096 x 16 x 32: 28 us, 77 TFLOP/s of 151.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
@@ -512,11 +510,22 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
     for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -off));
-      AtOperand<T> p;
-      at_operand(s[kb], p.w);
       sum = at_sum(s[kb], sum);
+      if constexpr (sizeof(T) == 2) {
+        unsigned w[8], v[8];
+        at_operand2(s[kb], w, v);
 #pragma unroll
-      for (int d = 0; d < NB; ++d) at_mma_tr<PC>(o[d], vt[buf], kb * 32, d * 32, p.w);
+        for (int d = 0; d < NB; ++d) {
+          const AtTr x = at_tr<PC>(vt[buf], kb * 32, d * 32);
+          at_mma_tr(o[d], x, w);
+          at_mma_tr(o[d], x, v);
+        }
+      } else {
+        AtOperand<T> p;
+        at_operand(s[kb], p.w);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) at_mma_tr<PC>(o[d], vt[buf], kb * 32, d * 32, p.w);
+      }
     }
   }
   sum = at_sum_halves(sum);

@@ -8,7 +8,7 @@ from tests import test_gpu_attention as T
 
 pytestmark = pytest.mark.gpu
 
-DTYPES, IDS = T.DTYPES[:1], T.IDS[:1]
+DTYPES, IDS = T.DTYPES, T.IDS
 A = T.A
 
 
