@@ -4,7 +4,7 @@
 #   build.sh --exp        a -DTAPIR_EXPERIMENTS build for tools/kbench.py (phase traces, experiment kernels) into
 #                         tools/bin/libtapir_hip_exp.so -- not next to the product library, never loaded by the package
 #                         unless TAPIR_HIP_LIB points at it
-#   build.sh --slp        the same sources WITH hipcc's SLP pass into tools/libtapir_hip_slp.so: the build that shows the hazard
+#   build.sh --slp        engine.hip WITH hipcc's SLP pass into tools/libtapir_hip_slp.so: the build that shows the hazard
 #                         below (tools/r06.sh, TAPIR_HIP_LIB=... pytest tests/test_gpu_cotenant.py fails with it); never shipped
 #
 # -fno-slp-vectorize, and the check behind the build: on MI355X `v_pk_fma_f32 ... op_sel:[0,1,0]` (low result from the HIGH
@@ -18,18 +18,24 @@
 set -e
 cd "$(dirname "$0")"
 BASE="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -fno-slp-vectorize"
-FLAGS="$BASE -shared"
+LINK="--offload-arch=gfx950 -fPIC -shared"
 # attention.hip: no packed-f32 arithmetic at all (its host pass warns that it does not know the feature)
 FLAGS_attention="-Xclang -target-feature -Xclang -packed-fp32-ops"
 FLAGS_engine=""
 if [ "$1" == "--exp" ]; then
   shift
-  mkdir -p ../../tools/bin
-  exec hipcc $FLAGS -DTAPIR_EXPERIMENTS engine.hip attention.hip -o ../../tools/bin/libtapir_hip_exp.so "$@"
+  mkdir -p ../../tools/bin build
+  hipcc $BASE $FLAGS_attention -DTAPIR_EXPERIMENTS -c attention.hip -o build/attention_exp.o "$@"
+  hipcc $BASE -DTAPIR_EXPERIMENTS -c engine.hip -o build/engine_exp.o "$@"
+  hipcc $LINK build/engine_exp.o build/attention_exp.o -o ../../tools/bin/libtapir_hip_exp.so
+  exec python3 check_packed_forms.py ../../tools/bin/libtapir_hip_exp.so 2
 fi
 if [ "$1" == "--slp" ]; then
   shift
-  exec hipcc ${FLAGS/ -fno-slp-vectorize/} engine.hip attention.hip -o ../../tools/libtapir_hip_slp.so "$@"
+  mkdir -p build
+  hipcc $BASE $FLAGS_attention -c attention.hip -o build/attention.o
+  hipcc ${BASE/ -fno-slp-vectorize/} -c engine.hip -o build/engine_slp.o "$@"
+  exec hipcc $LINK build/engine_slp.o build/attention.o -o ../../tools/libtapir_hip_slp.so
 fi
 # one object per translation unit, compiled side by side (build.sh --unit attention: that one only, then the link)
 UNITS="engine attention"
@@ -42,8 +48,8 @@ for u in $UNITS; do
   PIDS="$PIDS $!"
 done
 for p in $PIDS; do wait $p; done
-hipcc --offload-arch=gfx950 -fPIC -shared build/engine.o build/attention.o -o libtapir_hip.so
-python3 check_packed_forms.py libtapir_hip.so
+hipcc $LINK build/engine.o build/attention.o -o libtapir_hip.so
+python3 check_packed_forms.py libtapir_hip.so 2
 # the operators on torch tensors (host code: argument checks, autograd nodes)
 TORCH=$(python3 -c "import importlib.util, os; print(os.path.dirname(importlib.util.find_spec('torch').origin))")
 PYINC=$(python3 -c "import sysconfig; print(sysconfig.get_paths()['include'])")

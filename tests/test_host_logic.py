@@ -257,3 +257,31 @@ def test_the_built_library_has_no_high_half_selects_on_packed_f32_arithmetic():
   packed, bad = res
   assert packed > 10000, packed          # (the hand-packed kernels are there)
   assert not bad, bad
+
+
+def test_the_packed_forms_guard_reads_every_code_object():
+  """The library is linked from two units and holds a gfx950 code object of each: the guard has to see the engine's kernels and
+  the operators', whatever order the directory lists them in, and to fail where one is missing."""
+  import importlib.util
+  root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+  lib = os.path.join(root, 'tapnet_amd', 'csrc', 'libtapir_hip.so')
+  if not os.path.exists(lib):
+    pytest.skip('library not built')
+  spec = importlib.util.spec_from_file_location('check_packed_forms', os.path.join(root, 'tapnet_amd', 'csrc', 'check_packed_forms.py'))
+  mod = importlib.util.module_from_spec(spec)
+  spec.loader.exec_module(mod)
+  objects = mod.disassemble(lib)
+  if objects is None:
+    pytest.skip('llvm-objdump not installed')
+  assert len(objects) == 2
+  for kernel in ('mix_kernel', 'attn_fwd_kernel', 'layer_norm_bwd_kernel', 'rotary_rows_kernel'):
+    assert sum(kernel in dis for dis in objects) == 1, kernel
+  # (attention.hip is compiled without packed-f32 arithmetic)
+  operators = next(dis for dis in objects if 'attn_fwd_kernel' in dis)
+  assert not any(f'v_pk_{op}_f32' in operators for op in ('fma', 'mul', 'add'))
+  bad = {'a': 'x <first>:\n', 'b': 'x <second>:\n  v_pk_fma_f32 v[0:1], v[2:3], v[4:5], v[6:7] op_sel:[0,1,0]\n'}
+  for order in ('ab', 'ba'):
+    mod.disassemble = lambda _: [bad[n] for n in order]
+    assert mod.scan(lib) == (1, {'second': 1})
+    with pytest.raises(RuntimeError, match='code objects'):
+      mod.scan(lib, 1)
