@@ -174,17 +174,20 @@ int attn_check(tapir_ctx* c, const tapir_attn_args* a, bool backward) {
                     (long)a->batch * a->kv_heads * ((a->keys + AT_KEYS - 1) / AT_KEYS) <= most,
              TAPIR_ERR_UNSUPPORTED, "cross_attention: too many workgroups");
   const int epc = ctx_info(c).dtype == TAPIR_BF16 ? 8 : 4;
-  auto tensor_ok = [&](const void* p, const int64_t* st, bool empty) {
-    return empty || (p && aligned16(p) && st[0] % epc == 0 && st[1] % epc == 0 && st[2] % epc == 0);
+  // (an axis of one element has no stride: nothing steps over it)
+  auto tensor_ok = [&](const void* p, const int64_t* st, int64_t tokens, int heads) {
+    if (a->batch == 0 || tokens == 0) return true;
+    return p && aligned16(p) && (a->batch == 1 || st[0] % epc == 0) && (tokens == 1 || st[1] % epc == 0) && (heads == 1 || st[2] % epc == 0);
   };
   auto near = [](const int64_t* st) { return st[1] >= 0 && st[1] < AT_MAX_STRIDE; };
   OP_REQUIRE(c, a->queries <= 1 || (near(a->q_stride) && (!backward || near(a->dout_stride))), TAPIR_ERR_UNSUPPORTED,
              "cross_attention: tokens of q or dout are 2^22 elements apart or more, or in descending order");
   OP_REQUIRE(c, a->keys <= 1 || (near(a->k_stride) && near(a->v_stride)), TAPIR_ERR_UNSUPPORTED,
              "cross_attention: tokens of k or v are 2^22 elements apart or more, or in descending order");
-  const bool no_q = a->batch == 0 || a->queries == 0, no_k = a->batch == 0 || a->keys == 0;
-  OP_REQUIRE(c, tensor_ok(a->q, a->q_stride, no_q) && tensor_ok(a->k, a->k_stride, no_k) && tensor_ok(a->v, a->v_stride, no_k) &&
-                    (!backward || tensor_ok(a->dout, a->dout_stride, no_q)),
+  const bool no_q = a->batch == 0 || a->queries == 0;
+  OP_REQUIRE(c, tensor_ok(a->q, a->q_stride, a->queries, a->heads) && tensor_ok(a->k, a->k_stride, a->keys, a->kv_heads) &&
+                    tensor_ok(a->v, a->v_stride, a->keys, a->kv_heads) &&
+                    (!backward || tensor_ok(a->dout, a->dout_stride, a->queries, a->heads)),
              TAPIR_ERR_INVALID, "cross_attention: null tensor, or one whose rows do not start at multiples of 16 bytes");
   OP_REQUIRE(c, no_q || (a->out && aligned16(a->out)) || backward, TAPIR_ERR_INVALID, "cross_attention: null or misaligned output");
   if (backward) {

@@ -297,12 +297,12 @@ Tensor rotary_positions(const Tensor& x, const Tensor& positions_, const std::op
 
 // ----------------------------------------------------------------------------------------------------- cross attention
 // `t` itself where its rows (last axis) are dense, start at multiples of 16 bytes and are less than 2^22 elements apart, else a
-// dense copy
+// dense copy.  An axis of one element has no stride (torch calls such a tensor contiguous whatever number stands there).
 Tensor aligned(const Tensor& in) {
   Tensor t = plain(in);
   const int64_t epc = 16 / static_cast<int64_t>(t.element_size());
   bool good = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int d = 0; d < 3; ++d) good = good && t.stride(d) % epc == 0;
+  for (int d = 0; d < 3; ++d) good = good && (t.size(d) <= 1 || t.stride(d) % epc == 0);
   good = good && (t.size(1) <= 1 || t.stride(1) < (int64_t{1} << 22));
   if (good) return t;
   t = t.contiguous();

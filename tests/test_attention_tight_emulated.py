@@ -71,3 +71,18 @@ def test_the_bounds_reject_mistakes(dtype):
     ds = p * (D @ V.T - (D * (p @ V)).sum(-1, keepdim=True)) * dim ** -0.5
     shape = lambda t: t[None, :, None]
     assert all(rejected([shape(once(p) @ V), shape(once(ds) @ K), shape(once(ds).T @ Q), shape(once(p).T @ D)]))
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('queries,keys,heads,kv_heads', [(1, 1, 1, 1), (3, 1, 2, 1), (1, 5, 2, 2), (4, 70, 2, 1)])
+def test_axes_of_one_element_have_no_stride(dtype, queries, keys, heads, kv_heads):
+  """One clip, token or head sliced out of rows of an odd pitch: nothing steps over that axis."""
+  gen = torch.Generator().manual_seed(queries + keys)
+
+  def odd(tokens, heads):
+    t = torch.randn(1, tokens, heads, 32, generator=gen).to(dtype)
+    strides = [643, heads * 32 if tokens > 1 else 37, 32 if heads > 1 else 35, 1]
+    return t.as_strided(t.shape, strides)
+  q, k, v, dout = odd(queries, heads), odd(keys, kv_heads), odd(keys, kv_heads), odd(queries, heads)
+  with E.Ctx(dtype) as c:
+    compare(c, q, k, v, dout)

@@ -55,3 +55,24 @@ def test_rows_that_attend_to_everything(A, dtype, queries, keys, heads, kv_heads
   gen = T.generator(keys + queries)
   (_, k, v), dout = T.attention_inputs(gen, dtype, 1, queries, keys, heads, kv_heads, dim)
   compare(A, (0.3 * T.randn(gen, 1, queries, heads, dim)).to(dtype), k.detach(), v.detach(), dout)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_axes_of_one_element_have_no_stride(A, dtype):
+  """One clip, token or head sliced out of rows of an odd pitch, for every tensor and for the result's gradient."""
+  gen = T.generator(6)
+
+  def one_token():
+    t = T.randn(gen, 1, 1, 1, 35).to(dtype)[..., :32]
+    assert t.stride() == (35, 35, 35, 1)
+    return t
+
+  def one_head(tokens):
+    return T.randn(gen, 1, tokens, 3, 35).to(dtype)[:, :, :1, :32]
+
+  def one_clip(tokens, heads):
+    return T.randn(gen, 643 + tokens * heads * 32).to(dtype).as_strided((1, tokens, heads, 32), (643, heads * 32, 32, 1))
+  for q, k, v, dout in ((one_token(), one_token(), one_token(), one_token()), (one_token(), one_head(5), one_clip(5, 1), one_token()),
+                        (one_head(1), one_head(1), one_token(), one_head(1)), (one_clip(9, 4), one_clip(70, 2), one_clip(70, 2), one_clip(9, 4)),
+                        (one_head(4), one_clip(3, 1), one_head(3), one_head(4)), (one_clip(1, 4), one_clip(33, 4), one_clip(33, 4), one_clip(1, 4))):
+    compare(A, q, k, v, dout)
