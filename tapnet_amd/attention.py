@@ -14,7 +14,8 @@ pass is captured on a side stream, with no eager autograd graph of the same leav
 wait for the eager graph's stream inside the capture).  No kernel uses atomics: the same call gives the same bits, also where
 only some of the gradients are asked for.  Gradients are not differentiable again.
 
-The argument checks and autograd nodes are in ``csrc/torch_ops.cpp`` (built beside the library).
+The argument checks and autograd nodes are in ``csrc/torch_ops.cpp`` (built beside the library), which registers the operators with
+torch's dispatcher as ``torch.ops.tapnet_amd``: ``torch.jit.trace`` and ``make_fx`` record them, fake tensors get their shapes.
 """
 from __future__ import annotations
 
