@@ -79,6 +79,11 @@ void check_input(const char* name, const Tensor& t) {
   TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " has to be a dense tensor");
 }
 
+// No forward-mode derivatives: a tangent would be dropped without a word.
+void check_no_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "tapnet_amd.attention has no forward-mode derivatives, but ", name, " has a tangent");
+}
+
 void check_beside(const char* name, const Tensor& t, const Tensor& like, at::ScalarType type) {
   TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", the input on ", like.device());
   TORCH_CHECK_VALUE(t.scalar_type() == type, name, " has to be ", type, ", not ", t.scalar_type());
@@ -246,6 +251,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   check_input("x", x);
+  check_no_tangent("x", x);
+  check_no_tangent("weight", value(weight));
+  check_no_tangent("bias", value(bias));
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(value(weight)) || wants_grad(value(bias))))
     return LayerNorm::apply(x, weight, bias, eps);
   return norm_call(x, weight, bias, eps, false)[0];
@@ -334,6 +342,8 @@ Tensor rotary_positions(const Tensor& x, const Tensor& positions, at::OptionalIn
                         bool interleaved) {
   check_input("x", x);
   check_axes("x", x, 4);
+  check_no_tangent("x", x);
+  check_no_tangent("positions", positions);
   TORCH_CHECK_VALUE(!positions.requires_grad(), "positions have no gradient: detach them");
   std::vector<int64_t> sections;
   if (sections_.has_value()) {
@@ -525,6 +535,10 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
                        std::optional<double> scale_) {
   check_input("q", q);
   check_axes("q", q, 4);
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor&>("q", q), std::pair<const char*, const Tensor&>("k", k),
+                                std::pair<const char*, const Tensor&>("v", v)})
+    check_no_tangent(name, t);
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(1, q.size(3))));
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return CrossAttention::apply(q, k, v, lengths, mask, scale);
   return attn_call(q, k, v, lengths, mask, scale, false)[0];

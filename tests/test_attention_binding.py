@@ -2,6 +2,7 @@
 refused.  Tensors are on torch's meta device here; tests/test_gpu_attention_binding.py replays recordings on the GPU."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from tapnet_amd import attention as A
@@ -59,6 +60,22 @@ def test_recordings_hold_the_operators(name):
     targets = [str(n.target) for n in graph.graph.nodes if n.op == 'call_function']
     assert sum(t.startswith('tapnet_amd.' + name) for t in targets) == wanted, targets
     assert not any('empty' in t for t in targets), targets
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_tangents_are_refused(name):
+  """A tangent would be dropped: whichever tensor has it, with and without gradients."""
+  fn, inputs = calls(torch.float32)[name]
+  with fwd.dual_level():
+    for n in range(len(inputs)):
+      for grad in (False, True):
+        dual = [t.detach().requires_grad_(grad) for t in inputs]
+        dual[n] = fwd.make_dual(dual[n], torch.empty_like(dual[n]))
+        with pytest.raises(RuntimeError, match='forward-mode'):
+          fn(*dual)
+    positions = fwd.make_dual(meta(5, 3), meta(5, 3))
+    with pytest.raises(RuntimeError, match='forward-mode'):
+      A.rotary_positions(meta(2, 5, 4, 24), positions)
 
 
 def test_operators_below_autograd_check_what_they_get():
