@@ -439,7 +439,7 @@ int tapir_rotary_positions(tapir_ctx* ctx, const tapir_rotary_args* args, void* 
  * token, head) in elements, channels dense, every row at a multiple of 16 bytes, token strides of 0 to 2^22 - 1; dim a multiple of 8, at most 128;
  * scale > 0.  key_lengths [batch] int32 (device; clamped to 0 .. keys) and key_mask [batch, keys] bytes (nonzero = may be
  * attended to), either or both NULL: keys outside them are not read, whatever they hold.  A row without any key gives
- * zeros.  out [batch, queries, heads, dim] dense.  For a backward pass also out_f32 (the same, f32; f32 contexts may name
+ * zeros, one with keys but no softmax (all scores -inf, a NaN or +inf) NaN.  out [batch, queries, heads, dim] dense.  For a backward pass also out_f32 (the same, f32; f32 contexts may name
  * `out` itself) and stats [batch, kv_heads, heads / kv_heads * queries, 2] are written.
  * The backward pass takes the forward call's arguments (out may be NULL), dout (strides like q's) and writes dq and dk,
  * dv, dense (dq, or dk and dv together, may be NULL); rows of dk / dv outside the masks are zeros.  kv heads shared by

@@ -76,8 +76,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
   lengths from zero on, any strides (tensors whose rows are not dense or not at multiples of 16 bytes are copied).
   key_lengths: int32 ``[batch]``, the tokens of each clip (clamped to 0 .. keys; on the GPU, not read by the host).
   key_mask: bool ``[batch, keys]``, True where a token may be attended to.  Tokens outside either are not read: they may
-  hold anything, and their gradients are zeros.  A query without any token gives zeros.  scale: positive, default
-  ``dim ** -0.5``.
+  hold anything, and their gradients are zeros.  A query without any token gives zeros; one whose tokens' scores are all -inf, or hold a
+  NaN or +inf, gives NaN, as softmax does.  scale: positive, default ``dim ** -0.5``.
 
   Returns ``[batch, queries, heads, dim]`` in q's type.  Scores, statistics and sums are float32; in bfloat16 the
   probabilities and the scores' gradients enter the second products with 16 bits, twice bfloat16's eight.

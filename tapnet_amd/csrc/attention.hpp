@@ -415,6 +415,10 @@ template <typename T, int DP> struct AtWaves {
   static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
 };
 
+// 1 / l_r.  A row without keys: 0, its result and gradients are zeros.  A row that has keys but no positive sum -- all its scores are
+// -inf, or one is NaN or +inf -- has no softmax: NaN, for its result and for every gradient that it enters.
+__device__ __forceinline__ float at_inverse(float sum, bool keys) { return sum > 0.f ? 1.f / sum : keys ? NAN : 0.f; }
+
 // ---------------------------------------------------------------------------------------------------------------- forward
 // A workgroup: AT_QROWS query rows of one key head, `tiles_per_split` key tiles; two LDS buffers, the next tile's copies in
 // flight under the current tile's products.  A score costs the vector unit a multiply-add, an exponential (two issue slots), half a
@@ -453,6 +457,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
 #pragma unroll
   for (int d = 0; d < NB; ++d) o[d] = at_zero();
   float base = -INFINITY, sum = 0.f;   // base: of the exponentials, in powers of two
+  uint64_t some = 0;                   // (of any tile) there are keys at all
 
   AtStage<T, KT, DP> sk, sv;
   sk.init(a.ks[1]);
@@ -473,6 +478,7 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const uint64_t cur = bits;
+    some |= cur;
     dma_wait<0>();
     __syncthreads();
     if (t + 1 < t1) stage(t + 1, buf ^ 1);
@@ -538,10 +544,11 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         at_store4<float>(po + d * 32 + 8 * i + 4 * h, o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
-    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * ((bh * a.rows + row) * a.splits + split)) = make_float2(base, sum);
+    // (keys whose scores are all -inf: their sum of nothing is marked, for the join to tell it from a split without keys)
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * ((bh * a.rows + row) * a.splits + split)) = make_float2(base, some != 0 && sum == 0.f ? 1.f : sum);
     return;
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = at_inverse(sum, some != 0);
   const long at = (((long)b * a.Nq + query) * a.Hkv * a.G + head) * a.D;
 #pragma unroll
   for (int d = 0; d < NB; ++d)
@@ -575,6 +582,12 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
   for (int s = l; s < splits; s += 64) top = fmaxf(top, ml[s].x);
   top = wave_max(top);
   const float base = top == -INFINITY ? 0.f : top;
+  bool keys = true;
+  if (top == -INFINITY) {                       // no finite score: a row without keys, or one whose splits are marked
+    bool mine = false;
+    for (int s = l; s < splits; s += 64) mine = mine || ml[s].y != 0.f;
+    keys = __ballot(mine) != 0;
+  }
   const int c = (l % CG) * 4, g = l / CG;
   float sum = 0.f;
   float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -605,7 +618,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
       for (int i = 0; i < 4; ++i) x[i] += red[q][c + i];
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = at_inverse(sum, keys);
   const long at = ((b * a.Nq + row % a.Nq) * a.Hkv * a.G + hk * a.G + row / a.Nq) * a.D;
   if (g == 0 && c < a.D) {
     at_store4<T>((T*)a.out + at + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);

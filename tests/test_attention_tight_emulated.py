@@ -86,3 +86,34 @@ def test_axes_of_one_element_have_no_stride(dtype, queries, keys, heads, kv_head
   q, k, v, dout = odd(queries, heads), odd(keys, kv_heads), odd(keys, kv_heads), odd(queries, heads)
   with E.Ctx(dtype) as c:
     compare(c, q, k, v, dout)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('keys', [3, 2000])
+def test_rows_without_a_softmax(dtype, keys):
+  """A row whose allowed scores are all -inf, or hold a NaN or +inf, has no softmax: it is NaN and so is every gradient that it enters,
+  as of a sum over its terms.  Rows beside it, and rows whose other scores are -inf, keep their values; a clip whose mask leaves
+  nothing gives zeros."""
+  gen = torch.Generator().manual_seed(keys)
+  batch, queries, dim = 5, 4, 32
+  q, k, v, dout = E.inputs(gen, dtype, batch, queries, keys, 1, 1, dim)
+  k, v = k.contiguous(), v.contiguous()
+  big = 2.0 ** 80                                           # (its square is past float32's range)
+  q[:4, :, :, 0] = k[:4, :, :, 0] = 0.0
+  q[0, 1, 0, 0], k[0, :, 0, 0] = big, -big                  # all scores of one row -inf
+  q[1, 2, 0, 0], k[1, 0, 0, 0] = big, -big                  # one score of one row -inf
+  q[2, 0, 0, 0] = float('nan')
+  q[3, 3, 0, 0], k[3, -1, 0, 0] = big, big                  # one score of one row +inf
+  mask = torch.ones(batch, keys, dtype=torch.bool)
+  mask[4] = False
+  k[4] = float('nan')
+  with E.Ctx(dtype) as c:
+    out, dq, dk, dv = (t.float() for t in E.run_attention(c, q, k, v, None, mask, dout=dout))
+  lost = torch.zeros(batch, queries, dtype=torch.bool)
+  lost[0, 1] = lost[2, 0] = lost[3, 3] = True
+  assert torch.isnan(out[lost]).all() and torch.isnan(dq[lost]).all()
+  assert torch.isfinite(out[~lost]).all() and torch.isfinite(dq[1:][~lost[1:]]).all()
+  for b in (0, 2, 3):                                       # every key of the clip is a term of the row
+    assert torch.isnan(dk[b]).all() and torch.isnan(dv[b]).all()
+  assert torch.isfinite(dk[1]).all() and torch.isfinite(dv[1]).all()
+  assert all((t[4] == 0).all() for t in (out, dq, dk, dv))

@@ -76,3 +76,33 @@ def test_axes_of_one_element_have_no_stride(A, dtype):
                         (one_head(1), one_head(1), one_token(), one_head(1)), (one_clip(9, 4), one_clip(70, 2), one_clip(70, 2), one_clip(9, 4)),
                         (one_head(4), one_clip(3, 1), one_head(3), one_head(4)), (one_clip(1, 4), one_clip(33, 4), one_clip(33, 4), one_clip(1, 4))):
     compare(A, q, k, v, dout)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('keys', [3, 5000])
+def test_rows_without_a_softmax(A, dtype, keys):
+  """Rows whose allowed scores are all -inf, or hold a NaN or +inf: NaN, and every gradient that they enter; zeros where a mask
+  leaves nothing, whatever the tokens hold."""
+  gen = T.generator(keys)
+  (q, k, v), dout = T.attention_inputs(gen, dtype, 5, 4, keys, 1, 1, 32, packed=False)
+  big = 2.0 ** 80                                           # (its square is past float32's range)
+  with torch.no_grad():
+    q[:4, :, :, 0] = k[:4, :, :, 0] = 0.0
+    q[0, 1, 0, 0], k[0, :, 0, 0] = big, -big                # all scores of one row -inf
+    q[1, 2, 0, 0], k[1, 0, 0, 0] = big, -big                # one score of one row -inf
+    q[2, 0, 0, 0] = T.math.nan
+    q[3, 3, 0, 0], k[3, -1, 0, 0] = big, big                # one score of one row +inf
+    k[4] = T.math.nan
+  mask = torch.ones(5, keys, dtype=torch.bool, device='cuda')
+  mask[4] = False
+  y = A.cross_attention(q, k, v, key_mask=mask)
+  dq, dk, dv = (t.float() for t in T.grads_of(y, [q, k, v], dout))
+  out = y.detach().float()
+  lost = torch.zeros(5, 4, dtype=torch.bool, device='cuda')
+  lost[0, 1] = lost[2, 0] = lost[3, 3] = True
+  assert torch.isnan(out[lost]).all() and torch.isnan(dq[lost]).all()
+  assert torch.isfinite(out[~lost]).all() and torch.isfinite(dq[1:][~lost[1:]]).all()
+  for b in (0, 2, 3):
+    assert torch.isnan(dk[b]).all() and torch.isnan(dv[b]).all()
+  assert torch.isfinite(dk[1]).all() and torch.isfinite(dv[1]).all()
+  assert all((t[4] == 0).all() for t in (out, dq, dk, dv))
