@@ -437,7 +437,7 @@ int tapir_rotary_positions(tapir_ctx* ctx, const tapir_rotary_args* args, void* 
 /* softmax(scale q k^T) v of query rows over an encoder's tokens.  q [batch, queries, heads, dim], k and v [batch, keys,
  * kv_heads, dim], heads a multiple of kv_heads (query head j reads key head j / (heads / kv_heads)); strides (clip,
  * token, head) in elements, channels dense, every row at a multiple of 16 bytes, token strides of 0 to 2^22 - 1; dim a multiple of 8, at most 128;
- * scale > 0.  key_lengths [batch] int32 (device; clamped to 0 .. keys) and key_mask [batch, keys] bytes (nonzero = may be
+ * scale 2^-60 to 2^60.  key_lengths [batch] int32 (device; clamped to 0 .. keys) and key_mask [batch, keys] bytes (nonzero = may be
  * attended to), either or both NULL: keys outside them are not read, whatever they hold.  A row without any key gives
  * zeros, one with keys but no softmax (all scores -inf, a NaN or +inf) NaN.  out [batch, queries, heads, dim] dense.  For a backward pass also out_f32 (the same, f32; f32 contexts may name
  * `out` itself) and stats [batch, kv_heads, heads / kv_heads * queries, 2] are written.

@@ -77,7 +77,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
   key_lengths: int32 ``[batch]``, the tokens of each clip (clamped to 0 .. keys; on the GPU, not read by the host).
   key_mask: bool ``[batch, keys]``, True where a token may be attended to.  Tokens outside either are not read: they may
   hold anything, and their gradients are zeros.  A query without any token gives zeros; one whose tokens' scores are all -inf, or hold a
-  NaN or +inf, gives NaN, as softmax does.  scale: positive, default ``dim ** -0.5``.
+  NaN or +inf, gives NaN, as softmax does.  scale: 2^-60 to 2^60, default ``dim ** -0.5``.
 
   Returns ``[batch, queries, heads, dim]`` in q's type.  Scores, statistics and sums are float32; in bfloat16 the
   probabilities and the scores' gradients enter the second products with 16 bits, twice bfloat16's eight.

@@ -166,7 +166,8 @@ int attn_check(tapir_ctx* c, const tapir_attn_args* a, bool backward) {
   OP_REQUIRE(c, a->heads % a->kv_heads == 0, TAPIR_ERR_INVALID, "cross_attention: heads is not a multiple of kv_heads");
   OP_REQUIRE(c, a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0, TAPIR_ERR_UNSUPPORTED,
              "cross_attention: head dimension has to be a multiple of 8, at most 128");
-  OP_REQUIRE(c, a->scale > 0.f && isfinite(a->scale), TAPIR_ERR_INVALID, "cross_attention: scale has to be positive and finite");
+  // (dk / dv in bf16 begin their products at numbers of the size of a score over the scale: far from the ends of f32's range)
+  OP_REQUIRE(c, a->scale >= 0x1p-60f && a->scale <= 0x1p60f, TAPIR_ERR_INVALID, "cross_attention: scale has to be within 2^-60 .. 2^60");
   const long most = 1L << 30;   // rows, keys, and the workgroups of a launch stay below 2^31
   OP_REQUIRE(c, a->queries <= most && a->keys <= most && (long)a->heads * a->queries <= most && (long)a->batch * a->heads <= (1 << 20),
              TAPIR_ERR_UNSUPPORTED, "cross_attention: too many tokens or heads");

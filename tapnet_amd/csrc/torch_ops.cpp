@@ -397,8 +397,7 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Op
     TORCH_CHECK_VALUE(mask->dim() == 2 && mask->size(0) == batch && mask->size(1) == keys, "key_mask has to be bool [", batch, ", ", keys,
                       "], not ", mask->sizes());
   }
-  TORCH_CHECK_VALUE(scale > 0 && std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0,
-                    "scale has to be positive and finite, not ", scale);
+  TORCH_CHECK_VALUE(scale >= 0x1p-60 && scale <= 0x1p60, "scale has to be within 2^-60 .. 2^60, not ", scale);
 }
 
 tapir_attn_args attn_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Tensor& mask, double scale) {

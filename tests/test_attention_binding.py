@@ -108,3 +108,12 @@ def test_cpu_tensors_are_refused():
                lambda: A.layer_norm(q.requires_grad_()), lambda: A.cross_attention(q.requires_grad_(), k, k)):
     with pytest.raises(ValueError, match='GPU'):
       call()
+
+
+def test_scales_out_of_range_are_refused():
+  q = meta(1, 2, 2, 8)
+  for scale in (1.2e-38, 2.0 ** -61, 2.0 ** 61, 3e38, 1e39, float('nan'), float('inf')):
+    with pytest.raises(ValueError, match='scale'):
+      A.cross_attention(q, q, q, scale=scale)
+  for scale in (2.0 ** -60, 2.0 ** 60):
+    A.cross_attention(q, q, q, scale=scale)

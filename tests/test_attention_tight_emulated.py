@@ -117,3 +117,30 @@ def test_rows_without_a_softmax(dtype, keys):
     assert torch.isnan(dk[b]).all() and torch.isnan(dv[b]).all()
   assert torch.isfinite(dk[1]).all() and torch.isfinite(dv[1]).all()
   assert all((t[4] == 0).all() for t in (out, dq, dk, dv))
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('power', [-60, -30, 60])
+def test_scales_at_the_ends_of_the_range(dtype, power):
+  """Scores of ordinary size whose scale is far from one: the gradients are those of any other scale."""
+  gen = torch.Generator().manual_seed(3)
+  q, k, v, dout = E.inputs(gen, dtype, 1, 9, 900, 2, 1, 32)
+  scale = 2.0 ** power
+  q = (q.float() * 2.0 ** (-power - 2)).to(dtype)
+  with E.Ctx(dtype) as c:
+    got = E.run_attention(c, q, k, v, scale=scale, dout=dout)
+  want = N.attention(q, k, v, all_of(k), scale, dout)
+  for name, g, w in zip(('out', 'dq', 'dk', 'dv'), got, want[1:]):
+    N.check(name, g, w)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_scales_out_of_range_are_refused(dtype):
+  q = torch.zeros(1, 2, 1, 8, dtype=dtype)
+  with E.Ctx(dtype) as c:
+    for scale in (1.2e-38, 2.0 ** -61, 2.0 ** 61, 3e38, 0.0, -1.0):
+      a = E.attn_args(q, q, q, scale=scale)
+      a.out = a.out_f32 = a.stats = a.dout = a.dq = q.data_ptr()
+      for name in ('tapir_cross_attention', 'tapir_cross_attention_backward'):
+        assert c.raw(name, E.ctypes.byref(a), None) == E._ffi.TAPIR_ERR_INVALID
+        assert b'scale' in c.lib.tapir_last_error(c.ctx)
