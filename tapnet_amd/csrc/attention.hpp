@@ -30,6 +30,7 @@ constexpr int AT_QROWS = 32 * AT_WAVES;      // query rows of a forward / dq wor
 constexpr int AT_KEYS = 32 * AT_WAVES;       // keys of a dk / dv workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float AT_SLACK = 8.f;
+constexpr float AT_FAR = 0x1p24f, AT_NEAR = 0x1p10f;   // sizes of a base of the exponentials: at_exponent, attn_dkv_kernel
 constexpr long AT_MAX_STRIDE = 1L << 22;   // elements from token to token: offsets within a tile of 64 tokens stay below 2^30 bytes
 
 struct AttnArgs {
@@ -415,6 +416,15 @@ template <typename T, int DP> struct AtWaves {
   static constexpr int DKV = DP == 32 ? (BF16 ? 3 : 2) : DP == 64 ? 2 : 1;
 };
 
+// The exponent of p: s scale2 - m.  A fused multiply-add knows s scale2 beyond the bits of m, which is the rounded product of the
+// largest s: the largest p is 2^r, r up to half of m's last bit, and cancels from the normalised p.  From 2^31 on r would leave the
+// range of f32 (the sum was inf or 0): there, and already from AT_FAR on, the product is rounded first, as m was.
+__device__ __forceinline__ float at_exponent(float s, float scale2, float m) {
+#pragma clang fp contract(off)
+  const float product = s * scale2, rounded = product - m;
+  return fabsf(m) >= AT_FAR ? rounded : fmaf(s, scale2, -m);
+}
+
 // 1 / l_r.  A row without keys: 0, its result and gradients are zeros.  A row that has keys but no positive sum -- all its scores are
 // -inf, or one is NaN or +inf -- has no softmax: NaN, for its result and for every gradient that it enters.
 __device__ __forceinline__ float at_inverse(float sum, bool keys) { return sum > 0.f ? 1.f / sum : keys ? NAN : 0.f; }
@@ -512,10 +522,16 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_ke
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
     }
     const float off = base == -INFINITY ? 0.f : base;
+    const bool far = __ballot(fabsf(off) >= AT_FAR) != 0;
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
+      if (far) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -off));
+        for (int i = 0; i < 16; ++i) s[kb][i] = fast_exp2(at_exponent(s[kb][i], a.scale2, off));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = fast_exp2(fmaf(s[kb][i], a.scale2, -off));
+      }
       sum = at_sum(s[kb], sum);
       if constexpr (sizeof(T) == 2) {
         unsigned w[8], v[8];
@@ -699,6 +715,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
   for (int x = 0; x < CH / 2; ++x) { pin(qf[x]); pin(gf[x]); }
   pin(row_max);
   pin(row_inv);
+  const bool far = __ballot(fabsf(row_max) >= AT_FAR) != 0;
+  const float factor = far ? 1.f : a.scale2, offset = far ? 0.f : row_max;
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const uint64_t cur = bits;
@@ -718,8 +736,13 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kern
           g = at_mma(at_chunk<T, PC>(vt[buf], kb * 32 + (l & 31), 2 * x + h), gf[x], g, T{});
         }
       }
+      if (far) {
+        const float m = a.stats[2 * (bh * a.rows + (row < a.rows ? row : 0))];    // (read again: a register less on the usual way)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale2, -row_max)) * (BF16 ? g[i] : g[i] - delta);
+        for (int i = 0; i < 16; ++i) s[i] = at_exponent(s[i], a.scale2, m);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], factor, -offset)) * (BF16 ? g[i] : g[i] - delta);
       const unsigned mb = (unsigned)(cur >> (32 * kb));
       if (mb != 0xffffffffu) {
         const unsigned mine = mb >> (4 * h);
@@ -789,7 +812,11 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
   // m_r + log l_r), so that p = exp2(scale2 s) and ds = p dp remain; f32: m_r, D_r and 1 / l_r apart, because one number L_r would
   // be rounded at its own size (2^-21 at 10, a relative error of 5 u of the whole row).
   constexpr bool BF16 = sizeof(T) == 2;
-  __shared__ __attribute__((aligned(16))) float ld[2][BF16 ? 2 : 3][RT];
+  // bf16: where m_r is large (AT_NEAR), the products' sums would be rounded at the size of L_r and p be off by more than a bf16
+  // rounding: such steps, marked in `far`, form the scores again from zero and take m_r and log2(1 / l_r) apart, too (the test for it: 1 us of 276
+  // and 1.5 of 114 a training step).
+  __shared__ __attribute__((aligned(16))) float ld[2][BF16 ? 4 : 3][RT];
+  __shared__ unsigned far[2];
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, h = l >> 5;
   AtUnit unit;
   bool zero;
@@ -840,8 +867,15 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
     }
   };
   auto put_stats = [&](int buf) {
+    const uint64_t large = __ballot(threadIdx.x < RT && fabsf(row_stat.x) >= (BF16 ? AT_NEAR : AT_FAR));
+    if (threadIdx.x == 0) far[buf] = large != 0;      // (the rows are the first wave's)
     if (threadIdx.x < RT) {
-      if (BF16) ld[buf][0][threadIdx.x] = (log2f(row_stat.y) - row_stat.x) * unscale;   // (-inf for a row without keys: p = 0)
+      if (BF16) {
+        const float l = log2f(row_stat.y);                        // (-inf for a row without keys: p = 0)
+        ld[buf][0][threadIdx.x] = (l - row_stat.x) * unscale;
+        ld[buf][BF16 ? 2 : 0][threadIdx.x] = row_stat.x;
+        ld[buf][BF16 ? 3 : 0][threadIdx.x] = l;
+      }
       else { ld[buf][0][threadIdx.x] = row_stat.x; ld[buf][BF16 ? 0 : 2][threadIdx.x] = row_stat.y; }
     } else if (threadIdx.x < 2 * RT) {
       ld[buf][1][threadIdx.x - RT] = BF16 ? -row_stat.x : row_stat.x;
@@ -888,6 +922,8 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
       copy(t + 1, buf ^ 1);
       fetch((t + 2) * RT);
     }
+    const bool large = at_uniform(far[buf]) != 0;
+    const float factor = large ? 1.f : a.scale2;
     if constexpr (BF16) {
       // Operands are read from LDS a phase before the products that take them, and the fences keep it so: left to itself the
       // compiler reads each right before its product and waits (3 x 1000 x 8200 x 2 x 128: 119 -> 107 us).  64 and 96 channels
@@ -925,9 +961,19 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
         for (int d = 0; d < NB; ++d) qx[d] = at_tr<PC>(qt[buf], rb, d * 32);
         if ((DP == 32 || DP == 128) && rb + 32 < RT) read(rb + 32);
         sched_fence();
+        if (large) {
+          s = at_zero();
+#pragma unroll
+          for (int x = 0; x < CH / 2; ++x) s = at_mma(at_chunk<T, PC>(qt[buf], rb + (l & 31), 2 * x + h), kf[x], s, T{});
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = rb + 8 * (i >> 2) + 4 * h + (i & 3);
+            s[i] = at_exponent(s[i], a.scale2, ld[buf][BF16 ? 2 : 0][r]) + ld[buf][BF16 ? 3 : 0][r];
+          }
+        }
         AtOperand<T> p, e, f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = fast_exp2(s[i] * a.scale2);
+        for (int i = 0; i < 16; ++i) s[i] = fast_exp2(s[i] * factor);
         at_operand2(s, p.w, f.w);
 #pragma unroll
         for (int d = 0; d < NB; ++d) at_mma_tr(dv[d], gx[d], p.w);
@@ -952,9 +998,16 @@ __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_ke
           const tapir_f32x4 M = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][0][rb + 8 * i + 4 * h]);
           const tapir_f32x4 E = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][1][rb + 8 * i + 4 * h]);
           const tapir_f32x4 I = *reinterpret_cast<const tapir_f32x4*>(&ld[buf][2][rb + 8 * i + 4 * h]);
+          if (large) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[4 * i + j] = at_exponent(s[4 * i + j], a.scale2, M[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf(s[4 * i + j], a.scale2, -M[j]);
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[4 * i + j] = fast_exp2(fmaf(s[4 * i + j], a.scale2, -M[j])) * I[j];
+            s[4 * i + j] = fast_exp2(s[4 * i + j]) * I[j];
             g[4 * i + j] = s[4 * i + j] * (g[4 * i + j] - E[j]);
           }
         }

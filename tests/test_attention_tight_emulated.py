@@ -144,3 +144,36 @@ def test_scales_out_of_range_are_refused(dtype):
       for name in ('tapir_cross_attention', 'tapir_cross_attention_backward'):
         assert c.raw(name, E.ctypes.byref(a), None) == E._ffi.TAPIR_ERR_INVALID
         assert b'scale' in c.lib.tapir_last_error(c.ctx)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('power', [8, 12, 16, 20, 26, 32, 40, 60])
+@pytest.mark.parametrize('keys', [70, 3000])
+def test_huge_scores(dtype, power, keys):
+  """Scores of 2^power that are exact in float32 (small whole numbers times powers of two) and far apart: each row's softmax is one
+  token, or the mean of two whose scores are the same.  Nothing is rounded on the way, so that only the operands' own count."""
+  gen = torch.Generator().manual_seed(power)
+  q = torch.zeros(1, 6, 1, 16)
+  k = torch.zeros(1, keys, 1, 16)
+  q[0, :, 0, 0] = torch.tensor([1.0, -1.0, 2.0, -2.0, 3.0, 1.0])
+  k[0, :, 0, 0] = torch.randint(-100, 100, (keys,), generator=gen).float()
+  k[0, 17, 0, 0], k[0, keys - 1, 0, 0] = 120.0, 120.0
+  k[0, 3, 0, 0] = -127.0
+  k = k * 2.0 ** (power // 2)
+  q = q * 2.0 ** (power - power // 2)
+  v = torch.randint(-8, 9, (1, keys, 1, 16), generator=gen).float()
+  dout = torch.randint(-4, 5, (1, 6, 1, 16), generator=gen).float()
+  with E.Ctx(dtype) as c:
+    out, dq, dk, dv = (t.double() for t in E.run_attention(c, *(t.to(dtype) for t in (q, k, v)), scale=1.0, dout=dout.to(dtype)))
+  V, D = v[0, :, 0].double(), dout[0, :, 0].double()
+  p = torch.zeros(6, keys, dtype=torch.float64)
+  p[[0, 2, 4, 5], 17] = p[[0, 2, 4, 5], keys - 1] = 0.5
+  p[[1, 3], 3] = 1.0
+  ds = p * (D @ V.T - (D * (p @ V)).sum(-1, keepdim=True))
+  K, Q = k[0, :, 0].double(), q[0, :, 0].double()
+  # each result: its own rounding, and 2^-18 of the magnitudes in its sum (dp and D are sums of 16 products)
+  size = p * ((D.abs() @ V.abs().T) + (D.abs() * (p @ V.abs())).sum(-1, keepdim=True))
+  want = dict(out=(p @ V, p @ V.abs()), dq=(ds @ K, size @ K.abs()), dk=(ds.T @ Q, size.T @ Q.abs()), dv=(p.T @ D, p.T @ D.abs()))
+  for (name, (value, terms)), got in zip(want.items(), (out, dq, dk, dv)):
+    excess = (got[0, :, 0] - value).abs() - (N.rounded(value, 2.0 ** -18 * terms, dtype))
+    assert float(excess.nan_to_num(nan=float('inf')).max()) <= 0, (name, float(excess.max()))

@@ -106,3 +106,34 @@ def test_rows_without_a_softmax(A, dtype, keys):
     assert torch.isnan(dk[b]).all() and torch.isnan(dv[b]).all()
   assert torch.isfinite(dk[1]).all() and torch.isfinite(dv[1]).all()
   assert all((t[4] == 0).all() for t in (out, dq, dk, dv))
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('power', [8, 12, 16, 20, 26, 32, 60])
+@pytest.mark.parametrize('keys,dim', [(70, 16), (3000, 64), (20000, 128), (900, 96)])
+def test_huge_scores(A, dtype, power, keys, dim):
+  """Scores of 2^power that are exact in float32 and far apart: each row's softmax is one token, or the mean of two whose scores
+  are the same."""
+  gen = T.generator(power)
+  q, k = torch.zeros(1, 6, 1, dim, device='cuda'), torch.zeros(1, keys, 1, dim, device='cuda')
+  q[0, :, 0, 0] = torch.tensor([1.0, -1.0, 2.0, -2.0, 3.0, 1.0])
+  k[0, :, 0, 0] = torch.randint(-100, 100, (keys,), generator=gen, device='cuda').float()
+  k[0, 17, 0, 0], k[0, keys - 1, 0, 0] = 120.0, 120.0
+  k[0, 3, 0, 0] = -127.0
+  q, k = q * 2.0 ** (power - power // 2), k * 2.0 ** (power // 2)
+  v = torch.randint(-8, 9, (1, keys, 1, dim), generator=gen, device='cuda').float()
+  dout = torch.randint(-4, 5, (1, 6, 1, dim), generator=gen, device='cuda').float()
+  leaves = [t.to(dtype).requires_grad_() for t in (q, k, v)]
+  y = A.cross_attention(*leaves, scale=1.0)
+  got = [t.detach()[0, :, 0].double() for t in (y, *T.grads_of(y, leaves, dout.to(dtype)))]
+  Q, K, V, D = (t[0, :, 0].double() for t in (q, k, v, dout))
+  p = torch.zeros(6, keys, dtype=torch.float64, device='cuda')
+  p[[0, 2, 4, 5], 17] = p[[0, 2, 4, 5], keys - 1] = 0.5
+  p[[1, 3], 3] = 1.0
+  ds = p * (D @ V.T - (D * (p @ V)).sum(-1, keepdim=True))
+  # each result: its own rounding, and 2^-18 of the magnitudes in its sum (dp and D are sums of up to 128 exact products)
+  size = p * ((D.abs() @ V.abs().T) + (D.abs() * (p @ V.abs())).sum(-1, keepdim=True))
+  want = dict(out=(p @ V, p @ V.abs()), dq=(ds @ K, size @ K.abs()), dk=(ds.T @ Q, size.T @ Q.abs()), dv=(p.T @ D, p.T @ D.abs()))
+  for (name, (value, terms)), g in zip(want.items(), got):
+    excess = (g - value).abs() - N.rounded(value, 2.0 ** -18 * terms, dtype)
+    assert float(excess.nan_to_num(nan=T.math.inf).max()) <= 0, (name, float(excess.max()))
