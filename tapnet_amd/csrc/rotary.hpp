@@ -4,7 +4,7 @@
 //   (a, b) -> (a cos - b sin, a sin + b cos);   the gradient is the same map with -sin.
 // The two channels of a pair are neighbours (interleaved) or i and i + w / 2 of the section (halves).  Channels behind the last
 // section pass through.  Angles: turns = p * (base^(-2i/w) / 2 pi) in 64 bits (a product in 32 bits is off by 6e-3 at the
-// hundred-thousandth frame), reduced there to [-1/2, 1/2], sine and cosine of the rest in 32 bits.
+// hundred-thousandth frame), reduced there to an eighth of a turn, sine and cosine of the rest in 32 bits.
 #pragma once
 #include "common.hpp"
 
@@ -24,13 +24,12 @@ struct RotaryArgs {
   unsigned char axis[ROT_MAX_PAIRS], lo[ROT_MAX_PAIRS], hi[ROT_MAX_PAIRS];   // its axis and its two channels (< 256)
 };
 
-// cos and sin of 2 pi r.  r in turns: reduced to a quarter turn, then Taylor's polynomials on |t| <= pi/4 (first dropped
-// terms: t^10/10! < 2.5e-8 relative to cos, t^11/11! < 2e-9).
+// cos and sin of 2 pi r.  r in turns: reduced to a quarter turn and scaled in 64 bits, rounded once (half a step of t), then Taylor's
+// polynomials on |t| <= pi/4 (first dropped terms, absolute: t^10/10! < 2.5e-8, t^11/11! < 2e-9).  Off by less than 1.7 * 2^-24; with the
+// turn rounded to 32 bits before the reduction it was 2.3 * 2^-24.
 __device__ __forceinline__ void rot_sincos(double turns, float* sn, float* cs) {
-  const double w = turns - rint(turns);
-  const float r = (float)w;
-  const float k = rintf(4.f * r);
-  const float t = (r - 0.25f * k) * 6.28318530717958647692f;   // r - k/4 is exact
+  const double w = turns - rint(turns), k = rint(4.0 * w);
+  const float t = (float)((w - 0.25 * k) * 6.283185307179586476925286766559);   // w - k/4 is exact
   const float t2 = t * t;
   float s = 2.7557319e-6f;
   s = fmaf(s, t2, -1.9841270e-4f); s = fmaf(s, t2, 8.3333333e-3f); s = fmaf(s, t2, -1.6666667e-1f);
