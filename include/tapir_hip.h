@@ -404,7 +404,7 @@ int tapir_xconv_nt(tapir_ctx* ctx, const void* x, const void* wstream, const flo
 
 /* y = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis.  x [rows, channels] with `x_stride` elements from
  * row to row, y dense; gamma / beta [channels] or NULL (ones / zeros); mean, rstd [rows] are written where both are
- * given (the backward pass needs them).  Any channel count; rows of whole 16-byte multiples that start at such
+ * given (the backward pass needs them).  Up to 2^30 channels; rows of whole 16-byte multiples that start at such
  * addresses are read and written 16 bytes at a time. */
 int tapir_layer_norm(tapir_ctx* ctx, const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y,
                      float* mean, float* rstd, int64_t rows, int channels, float eps, void* stream);

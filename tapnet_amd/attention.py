@@ -47,7 +47,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
   """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis, as the norms of the PIPs mixer (scale only,
   tapnet/models/tapir_model.py:70-77) and of ExtraConvs (:176) have it, for any shape, and with gradients.
 
-  x: float32 or bfloat16 ``[..., channels]`` of any strides.  weight, bias: float32 ``[channels]`` or None.  Statistics
+  x: float32 or bfloat16 ``[..., channels]`` of any strides, at most 2^30 channels.  weight, bias: float32 ``[channels]`` or None.  Statistics
   and sums are float32; the result has x's type.  Gradients of x (its type), weight and bias (float32)."""
   return _ops().layer_norm(x, weight, bias, eps)
 

@@ -274,6 +274,7 @@ int tapir_layer_norm(tapir_ctx* c, const void* x, int64_t x_stride, const float*
   if (!c) return TAPIR_ERR_INVALID;
   const CtxInfo ci = ctx_info(c);
   OP_REQUIRE(c, rows >= 0 && channels >= 1 && eps >= 0.f && isfinite(eps), TAPIR_ERR_INVALID, "layer_norm: bad size or eps");
+  OP_REQUIRE(c, channels <= LN_MAX_CHANNELS, TAPIR_ERR_UNSUPPORTED, "layer_norm: more than 2^30 channels");
   OP_REQUIRE(c, (mean == nullptr) == (rstd == nullptr), TAPIR_ERR_INVALID, "layer_norm: mean and rstd go together");
   if (rows == 0) return TAPIR_OK;
   OP_REQUIRE(c, x && y, TAPIR_ERR_INVALID, "layer_norm: null tensor");
@@ -290,6 +291,7 @@ int tapir_layer_norm(tapir_ctx* c, const void* x, int64_t x_stride, const float*
 int tapir_layer_norm_workspace(tapir_ctx* c, int64_t rows, int channels, uint64_t* bytes) {
   if (!c) return TAPIR_ERR_INVALID;
   OP_REQUIRE(c, bytes && rows >= 0 && channels >= 1, TAPIR_ERR_INVALID, "layer_norm: bad size");
+  OP_REQUIRE(c, channels <= LN_MAX_CHANNELS, TAPIR_ERR_UNSUPPORTED, "layer_norm: more than 2^30 channels");
   const int v = ctx_info(c).dtype == TAPIR_BF16 ? 8 : 4;
   const unsigned shares = std::max(ln_bwd_grid(rows, channels, 1), ln_bwd_grid(rows, channels, v));
   *bytes = (uint64_t)shares * 2 * ln_part_stride(channels) * sizeof(float);
@@ -302,6 +304,7 @@ int tapir_layer_norm_backward(tapir_ctx* c, const void* x, int64_t x_stride, con
   if (!c) return TAPIR_ERR_INVALID;
   const CtxInfo ci = ctx_info(c);
   OP_REQUIRE(c, rows >= 0 && channels >= 1, TAPIR_ERR_INVALID, "layer_norm: bad size");
+  OP_REQUIRE(c, channels <= LN_MAX_CHANNELS, TAPIR_ERR_UNSUPPORTED, "layer_norm: more than 2^30 channels");
   OP_REQUIRE(c, rows == 0 || (x && dy && mean && rstd), TAPIR_ERR_INVALID, "layer_norm: null tensor");
   const int ept = ln_ept(ci.dtype, channels, x_stride, x, dy_stride, dy, dx);
   const unsigned grid = ln_bwd_grid(rows, channels, ept);

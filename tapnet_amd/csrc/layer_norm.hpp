@@ -14,6 +14,7 @@
 namespace tapir {
 
 constexpr int LN_THREADS = 256;
+constexpr int LN_MAX_CHANNELS = 1 << 30;   // columns are counted in 32 bits, a stride of threads past the last one included
 constexpr int LN_REDUCE_COLS = 16;   // columns per workgroup of the partial sums' reduction
 
 // columns of a row of partial sums: every row starts at a multiple of 16 bytes

@@ -151,7 +151,7 @@ Rows as_rows(const Tensor& in) {
 void check_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
   check_input("x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x has to have a last axis of at least one channel");
-  TORCH_CHECK_VALUE(x.size(-1) < (int64_t{1} << 31), "x has too many channels");
+  TORCH_CHECK_VALUE(x.size(-1) <= (int64_t{1} << 30), "x has more than 2^30 channels");
   for (const auto& [name, p] : {std::pair<const char*, const OptTensor&>("weight", weight), std::pair<const char*, const OptTensor&>("bias", bias)}) {
     if (!p.has_value()) continue;
     check_beside(name, *p, x, at::kFloat);

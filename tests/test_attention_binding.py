@@ -117,3 +117,9 @@ def test_scales_out_of_range_are_refused():
       A.cross_attention(q, q, q, scale=scale)
   for scale in (2.0 ** -60, 2.0 ** 60):
     A.cross_attention(q, q, q, scale=scale)
+
+
+def test_layer_norm_channels_past_32_bits_are_refused():
+  with pytest.raises(ValueError, match='channels'):
+    A.layer_norm(meta(2 ** 30 + 1))
+  assert A.layer_norm(meta(2 ** 30)).shape == (2 ** 30,)

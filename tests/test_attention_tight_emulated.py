@@ -192,3 +192,16 @@ def test_rotary_sines_and_cosines():
   angle = positions.double()[:, 0]
   worst = max(float((y[:, 0] - angle.cos()).abs().max()), float((y[:, 1] - angle.sin()).abs().max()))
   assert worst <= 1.7 * 2.0 ** -24, worst * 2 ** 24
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_layer_norm_channels_past_32_bits_are_refused(dtype):
+  """Columns are counted in 32 bits, a stride of threads past the last one included: from 2^30 on nothing is launched."""
+  p, nbytes = torch.zeros(64).data_ptr(), E.ctypes.c_uint64()
+  with E.Ctx(dtype) as c:
+    for channels in (2 ** 30 + 1, 2 ** 31 - 256, 2 ** 31 - 1):
+      for rc in (c.raw('tapir_layer_norm_workspace', 0, channels, E.ctypes.byref(nbytes)),
+                 c.raw('tapir_layer_norm', p, channels, None, None, p, None, None, 0, channels, 1e-5, None),
+                 c.raw('tapir_layer_norm_backward', p, channels, p, channels, None, p, p, p, None, None, 0, channels, None, 0, None)):
+        assert rc == E._ffi.TAPIR_ERR_UNSUPPORTED
+    assert c.raw('tapir_layer_norm_workspace', 1, 2 ** 30, E.ctypes.byref(nbytes)) == 0
