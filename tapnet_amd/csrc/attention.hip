@@ -96,19 +96,21 @@ struct AttnPlan {
 
 size_t round4(size_t n) { return (n + 3) & ~(size_t)3; }   // (shares of a workspace start at multiples of 16 bytes)
 
-// Splits of a long axis: `base` workgroups of `steps` steps each become base * s of steps / s, joined at `join` us a split.  The s of
-// the least estimated time is taken.  Estimate: n workgroups that share a compute unit (of 256) take t1 max(1 + (n - 1) / 2, 0.7 n)
-// a step (24576 keys x 64, forward: 1.11, 1.74, 2.49 us for 1 to 3), `occupancy` of them at once, and three
-// steps' time to begin.  Measured, 256 x 49152 x 4 x 64: forward 699 us unsplit, 34 / 30 / 32 / 34 / 39 us for 256 / 512 / 768 / 1024 /
-// 1536 workgroups; 3 x 1000 x 8200 x 2 x 128: backward 169 us with the rows of dk / dv unsplit, 189 / 202 / 224 us with 2 / 3 / 6 splits.
-struct AttnSplit { long steps, base; int occupancy; double t1, join, join_first; };
+// Splits of a long axis: `base` workgroups (or `other`, as likely) of `steps` steps each become base * s of steps / s, joined at `join` us
+// a split.  The s of the least estimated time is taken.  Estimate: n workgroups that share a compute unit (of 256) take
+// t1 max(1 + (n - 1) / 2, 0.7 n) a step (24576 keys x 64, forward: 1.11, 1.74, 2.49 us for 1 to 3), `occupancy` of them at once, and three
+// steps' time to begin.  Measured, 256 x 49152 x 4 x 64, one part of p: forward 699 us unsplit, 34 / 30 / 32 / 34 / 39 us for 256 / 512 /
+// 768 / 1024 / 1536 workgroups; keys of the forward pass and of dq, 3 x 1000 x 8200, 4 / 2 heads x 128, half full: training step 428 / 329 /
+// 279 / 272 us with the forward pass in 1 / 2 / 4 / 8 splits, 476 / 346 / 282 / 274 with dq in as many (and the rows of dk / dv in two).
+struct AttnSplit { long steps, base, other; int occupancy; double t1, join, join_first; };
 void attn_split(const AttnSplit& x, int* splits, int* per_split) {
   double best = 0;
   *splits = 0;
   auto shared = [&](long n) { return n == 0 ? 0.0 : x.t1 * std::max(1 + 0.5 * (n - 1), 0.7 * n); };
   for (long s = 1, per = x.steps;; ) {
-    const long n = (x.base * s + 255) / 256, full = n / x.occupancy;
-    const double t = (per + 3) * (full * shared(x.occupancy) + shared(n % x.occupancy)) + (s > 1 ? x.join_first + x.join * s : 0);
+    const long n = (x.base * s + 255) / 256;
+    auto rounds = [&](long n) { return n / x.occupancy * shared(x.occupancy) + shared(n % x.occupancy); };
+    const double t = (per + 3) * 0.5 * (rounds(n) + rounds((x.other * s + 255) / 256)) + (s > 1 ? x.join_first + x.join * s : 0);
     if (*splits == 0 || t < best) { best = t; *splits = (int)s; *per_split = (int)per; }
     if (per == 1 || n > 2 * x.occupancy) break;
     --per;                                        // the next number of splits that shortens them
@@ -136,7 +138,7 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
   const double row_bytes = 8.0 * heads * rows * p.dp, key_bytes = 16.0 * heads * a->keys * p.dp;   // written and read
   // (a padded batch is taken to hold two thirds of its tokens: the lengths themselves are on the device)
   auto filled = [&](long units) { return std::max<long>(1, a->key_lengths ? units * 2 / 3 : units); };
-  const AttnSplit keys{tiles, filled(heads * p.row_tiles), backward ? dq_occ[bf16][w] : fwd_occ[bf16][w],
+  const AttnSplit keys{tiles, filled(heads * p.row_tiles), filled(heads * p.row_tiles), backward ? dq_occ[bf16][w] : fwd_occ[bf16][w],
                        backward ? dq_us[bf16][w] : fwd_us[bf16][w], row_bytes * us_per_byte, backward ? 3.0 : 4.0};
   attn_split(keys, &p.splits, &p.tiles_per_split);
   if (!backward) {
@@ -148,7 +150,13 @@ AttnPlan attn_plan(const tapir_attn_args* a, int dtype, bool backward) {
     return p;
   }
   const int rt = attn_row_step(dtype, p.dp);
-  const AttnSplit by_row{std::max<long>(1, (rows + rt - 1) / rt), filled(heads * ((a->keys + AT_KEYS - 1) / AT_KEYS)),
+  // Split rows mean f32 shares of dk and dv for every key, which pays only where compute units would be idle: a padded batch is
+  // estimated at half and at two thirds of its tokens, so that one guess just past a whole number of rounds does not buy a split.  3 x
+  // 1000 x 8200, 4 / 2 heads x 128, half full (195 units; 260 at two thirds): training step 249 us unsplit, 273 / 289 with 2 / 3 splits.  Where
+  // units are few, splits stay: 3 x 3000 x 1000 x 2 x 128: 223 / 156 / 121 / 110 / 104 us with 1 / 2 / 4 / 6 / 8; 2 x 700 x 5000 x 2 x 96: 107 / 97 /
+  // 108 with 1 / 2 / 3.
+  const long key_units = heads * ((a->keys + AT_KEYS - 1) / AT_KEYS);
+  const AttnSplit by_row{std::max<long>(1, (rows + rt - 1) / rt), filled(key_units), a->key_lengths ? std::max<long>(1, key_units / 2) : filled(key_units),
                          dkv_occ[bf16][w], dkv_us[bf16][w], key_bytes * us_per_byte, p.splits > 1 ? 1.0 : 3.0};
   attn_split(by_row, &p.row_splits, &p.row_steps_per_split);
   p.delta = round4((size_t)heads * rows);

@@ -205,3 +205,22 @@ def test_layer_norm_channels_past_32_bits_are_refused(dtype):
                  c.raw('tapir_layer_norm_backward', p, channels, p, channels, None, p, p, p, None, None, 0, channels, None, 0, None)):
         assert rc == E._ffi.TAPIR_ERR_UNSUPPORTED
     assert c.raw('tapir_layer_norm_workspace', 1, 2 ** 30, E.ctypes.byref(nbytes)) == 0
+
+
+def test_rows_of_a_padded_batch_are_not_split_on_a_guess():
+  """Shares of dk and dv cost their memory and a join for every key, the padding's too: a padded batch that has nearly a tile for every
+  compute unit goes without (the workspace tells), as the whole batch does; one with few tiles keeps them."""
+  def shares(batch, queries, keys, heads, kv_heads, dim, padded):
+    a = E._ffi.TapirAttnArgs(batch, queries, keys, heads, kv_heads, dim, 0.1)
+    a.key_lengths = 16 if padded else None          # (not read)
+    out = []
+    with E.Ctx(torch.bfloat16) as c:
+      for dk in (None, 16):
+        a.dq, a.dk, a.dv, n = 16, dk, dk, E.ctypes.c_uint64()
+        c('tapir_cross_attention_workspace', E.ctypes.byref(a), 1, E.ctypes.byref(n))
+        out.append(n.value)
+    return (out[1] - out[0]) // (8 * batch * keys * kv_heads * dim)
+  assert shares(3, 1000, 8200, 4, 2, 128, True) == 0
+  assert shares(3, 1000, 8200, 4, 2, 128, False) == 0
+  assert shares(1, 40000, 4096, 1, 1, 64, False) > 1
+  assert shares(3, 40000, 4096, 1, 1, 64, True) > 1 and shares(3, 3000, 1000, 2, 2, 128, True) > 4
