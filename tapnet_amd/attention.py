@@ -81,5 +81,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
 
   Returns ``[batch, queries, heads, dim]`` in q's type.  Scores, statistics and sums are float32; in bfloat16 the
   probabilities and the scores' gradients enter the second products with 16 bits, twice bfloat16's eight.
-  In float32 the result itself is kept for the backward pass, as softmax keeps its own: overwriting it in place is an error there."""
+  In float32 the result itself is kept for the backward pass, as softmax keeps its own: overwriting it in place is an error there.
+  The gradients of q and k use the rounded result (``sum(grad * out)`` of a row): in float32, where one token dominates a row, they
+  are up to 2.2 times as far from the exact ones as a form that sums over the tokens again, some 1e-6 of their size."""
   return _ops().cross_attention(q, k, v, key_lengths, key_mask, scale)

@@ -54,8 +54,9 @@ struct AttnArgs {
   float scale, scale2;                 // scale, scale * log2(e)
 };
 
-// physical 16-byte chunk of logical chunk c in row r of a tile with CH chunks a row: eight consecutive rows reading the same
-// chunk, and four consecutive rows reading a pair of chunks, each touch all banks once.
+// physical 16-byte chunk of logical chunk c in row r of a tile with CH chunks a row: rows that are read together have their chunks in
+// different places of a bank line.  Measured conflict cycles, of the cycles in which LDS works: a third at 32 and 64 channels (dq 0.40, dk / dv
+// 0.24), 0.44 to 0.49 at 128; f32 0.18 to 0.29.  LDS works in 2 to 31 % of a compute unit's busy cycles and bounds none of these kernels.
 template <int CH> __device__ __forceinline__ int at_swizzle(int r, int c) {
   if (CH >= 8) return c ^ (((r & 3) << 1) | ((r >> 2) & 1));
   return c ^ ((r & 2) | ((r >> 2) & 1));        // 64-byte rows: the row's parity picks the half of a bank line already
@@ -433,8 +434,9 @@ __device__ __forceinline__ float at_inverse(float sum, bool keys) { return sum >
 // A workgroup: AT_QROWS query rows of one key head, `tiles_per_split` key tiles; two LDS buffers, the next tile's copies in
 // flight under the current tile's products.  A score costs the vector unit a multiply-add, an exponential (two issue slots), half a
 // maximum, an addition and three operations that split it in two parts (and, subtract, half a conversion, half a permutation): bound by
-// that next to three products.  Three waves a SIMD at 64 channels hold the operands (161 registers; at four they spill: 373 us
-// for 337).  4096 x 49152 x 4 x 64, bf16: 337 us with the join, 0.92 PFLOP/s executed; f32 256 x 4096 x 16 x 32: 28 us, 77 TFLOP/s of 151.
+// that (0.74 of the vector unit's cycles) next to three products (0.45 of the matrix unit's).  Three waves a SIMD at 64 channels hold the
+// operands (158 registers; at four they spill: 373 us for 337).  4096 x 49152 x 4 x 64, bf16: 334-337 us with the join, 0.92 PFLOP/s
+// executed (the kernel alone 337 to 427 us, median 348, under the profiler's trace); f32 2 x 256 x 4096 x 8 x 32: 28.6 us, 75 TFLOP/s of 151.
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::FWD)) void attn_fwd_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
@@ -647,7 +649,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_join_kernel(AttnArgs a) {
 // dq (and D_r on the way): the forward kernel's loop with p from the saved statistics; 1 / l_r is a factor of the whole row and
 // joins it at the end.  Keys are split like the forward pass': with few rows there are too few row tiles to fill the chip (256 rows of
 // 4 heads are 8 workgroups: 1.2 ms unsplit).  Bound by matrix and vector instructions in turn (S, dP, two parts of dQ: 256 x 49152 x
-// 4 x 64, bf16: 35-39 us, 0.7 PFLOP/s executed; f32 256 x 4096 x 16 x 32: 37 us, 85 TFLOP/s).
+// 4 x 64, bf16: 40 us, 0.65 PFLOP/s executed; f32 2 x 256 x 4096 x 8 x 32: 40 us, 80 TFLOP/s; matrix unit 0.35 and 0.60 busy).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DQ)) void attn_dq_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, KT = AtTile<T>::KT, NB = DP / 32;
@@ -802,7 +804,7 @@ __global__ __launch_bounds__(AT_THREADS) void attn_delta_kernel(AttnArgs a) {
 // dk, dv: a workgroup AT_KEYS keys of one key head, all query rows of the group's heads (or a split of them), RT at a time.
 // Six products a step in bf16 (S, dP and two parts each of dV and dK).  K and V stay in registers as operands, dK and dV as sums: two
 // waves a SIMD at 64 channels, one at 128.  Bound by matrix instructions for many rows (4096 x 49152: 1.0 PFLOP/s executed with dq), by
-// loading and storing its keys for few (256 rows are four steps; 49152 x 4 x 64: 56-63 us).
+// loading and storing its keys for few (256 rows are four steps; 49152 x 4 x 64: 64 us, matrix unit 0.31 busy).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, (AtWaves<T, DP>::DKV)) void attn_dkv_kernel(AttnArgs a) {
   constexpr int EPC = AtFrag<T>::EPC, CH = DP / EPC, PC = AtPitch<T, DP>::V, NB = DP / 32, RT = AtRowTile<T, DP>::RT;

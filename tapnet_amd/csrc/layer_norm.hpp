@@ -6,8 +6,9 @@
 // One pass over memory: a row stays in the registers of LPR lanes (NCH chunks of EPT elements each) between its statistics and
 // its output, so x is read once and y written once.  Statistics are two sums in f32 over those registers (mean first, then the
 // squares of the centred values: no cancellation).  Bound: HBM, 2 x (forward) and 3 x (backward) the tensor's bytes.  49152 x 256 bf16:
-// forward 9.5 us = 5.3 TB/s (21 us before the next rows were fetched under this step's sums), backward 15.5 us = 4.9 TB/s and 3.5 us for
-// the shares of the parameters' gradients; 12288 x 512 f32: 9 + 14.5 + 3.5 us.
+// forward 10.3 us = 4.9 TB/s (21 us before the next rows were fetched under this step's sums), backward 15.9 us = 4.7 TB/s and 3.9 us for
+// the shares of the parameters' gradients; 12288 x 512 f32: 10.0 + 14.6 + 3.4 us.  Rows stay in registers up to 2048 channels in aligned
+// bf16 and 1024 otherwise; longer ones are read three times (layer_norm_long_kernel, layer_norm_bwd_long_kernel: twice, column sums in memory).
 #pragma once
 #include "common.hpp"
 

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryArgs a) {
 // The same, 16 bytes a lane: D / EPC lanes hold a row, a wave R = 64 / (D / EPC) tokens.  A lane works out the cosines and sines of
 // its channels once and takes `heads` heads with them, ROT_HEADS at a time: their loads are in flight together, each row goes
 // through LDS once (the other channel of a pair lies anywhere in it) and is stored in whole lanes.  Bound: HBM, the tensor read and
-// written once: 2 x 49152 x 4 x 64 bf16 22 us = 4.6 TB/s (35 us with two bytes a lane).
+// written once: 2 x 49152 x 4 x 64 bf16 22.9 us = 4.4 TB/s (35 us with two bytes a lane).
 constexpr int ROT_HEADS = 4;
 
 struct RotaryRowArgs {
