@@ -11,8 +11,9 @@ Calls are enqueued on the current stream of the tensors' device, whatever the cu
 Scratch memory comes from torch's allocator, so calls on several streams and captured graphs do not share any.  A graph
 may capture them once a call of the same element type has been made on the device (it prepares the library); a backward
 pass is captured on a side stream, with no eager autograd graph of the same leaves alive (torch's autograd engine would
-wait for the eager graph's stream inside the capture).  No kernel uses atomics: the same call gives the same bits, also where
-only some of the gradients are asked for.  Gradients are not differentiable again, and forward-mode tangents are refused (RuntimeError).
+wait for the eager graph's stream inside the capture; refused where such a leaf is an operator's input).  No kernel uses
+atomics: the same call gives the same bits, also where only some of the gradients are asked for.  Gradients are not
+differentiable again, and forward-mode tangents are refused (RuntimeError).
 
 The argument checks and autograd nodes are in ``csrc/torch_ops.cpp`` (built beside the library), which registers the operators with
 torch's dispatcher as ``torch.ops.tapnet_amd``: ``torch.jit.trace`` and ``make_fx`` record them, fake tensors get their shapes.

@@ -9,6 +9,7 @@
 // behind the dispatcher would be recorded as an uninitialised allocation and nothing else.
 #include <ATen/DeviceGuard.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPFunctions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -110,6 +111,29 @@ Tensor workspace(uint64_t bytes, const Tensor& like) {
 // The registered operator `name`, as a C++ function.
 template <class Fn> c10::TypedOperatorHandle<Fn> registered(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
+}
+
+// A leaf's accumulation node belongs to the stream on which it was made.  Where a backward pass is captured while an eager graph of the
+// same leaf is alive, torch's engine would make that stream, which is not part of the capture, wait for the captured gradient; the error
+// comes up on the engine's own thread and ends the process.  Said here, before the gradient is handed on, it is an error of the call.
+void check_capture(const Tensor& like) {
+  if (!like.is_cuda() || c10::hip::device_count() == 0) return;      // (a recorded program's tensors)
+  const hipStream_t stream = current_stream(like);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr) return;
+  for (const auto& edge : node->next_edges()) {
+    if (edge.function == nullptr || edge.function->name() != "torch::autograd::AccumulateGrad") continue;
+    const auto of_leaf = edge.function->stream();
+    if (!of_leaf.has_value()) continue;
+    const hipStream_t other = c10::hip::HIPStreamMasqueradingAsCUDA(*of_leaf).stream();
+    if (other == stream) continue;
+    const hipError_t rc = hipStreamIsCapturing(other, &status);
+    if (rc != hipSuccess) (void)hipGetLastError();
+    TORCH_CHECK(rc == hipSuccess && status == hipStreamCaptureStatusActive,
+                "a backward pass is captured while an eager autograd graph of the same leaf is alive: delete its results first");
+  }
 }
 
 // Gradients are not differentiable again: asked for a second derivative, the node behind them says so.
@@ -234,6 +258,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = registered<decltype(norm_backward)>("tapnet_amd::layer_norm_backward");
+    check_capture(grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     // (the node's edges are those of the tensors that were given)
     const bool has_weight = saved[1].defined(), has_bias = ctx->saved_data["bias"].toBool();
@@ -331,6 +356,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture(grads[0]);
     variable_list out(5);
     out[0] = turn_call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["sections"].toIntVector(),
                        ctx->saved_data["bases"].toDoubleVector(), ctx->saved_data["interleaved"].toBool(), true);
@@ -516,6 +542,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = registered<decltype(attn_backward)>("tapnet_amd::cross_attention_backward");
+    check_capture(grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const bool want_q = ctx->needs_input_grad(0), want_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     variable_list out(6);

@@ -73,3 +73,30 @@ def test_checkpointed(A):
   want = torch.autograd.grad(fn(*leaves), leaves, dout)
   got = torch.autograd.grad(checkpoint(fn, *leaves, use_reentrant=False), leaves, dout)
   assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'rotary_positions', 'cross_attention'])
+def test_a_backward_pass_captured_over_a_live_eager_graph_is_refused(A, name):
+  """An error of the call, not the end of the process; without the eager graph the same capture works."""
+  gen = T.generator(9)
+  x = T.randn(gen, 1, 6, 2, 32).requires_grad_()
+  k, at, dy = T.randn(gen, 1, 9, 2, 32), torch.rand(6, 2, generator=gen, device='cuda'), T.randn(gen, 1, 6, 2, 32)
+  fn = {'layer_norm': lambda: A.layer_norm(x), 'rotary_positions': lambda: A.rotary_positions(x, at),
+        'cross_attention': lambda: A.cross_attention(x, k, k)}[name]
+  step = lambda: torch.autograd.grad(fn(), [x], dy)[0]
+  want = step()
+  alive = fn()
+  print('capture over a live eager graph', flush=True)
+  with pytest.raises(RuntimeError, match='eager autograd graph'):
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+      step()
+  torch.cuda.synchronize()
+  del alive
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    got = step()
+  for _ in range(3):
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
